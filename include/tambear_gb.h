@@ -138,7 +138,12 @@ tbgb_status tbgb_groupby_dense(tbgb_ctx* ctx, const int32_t* d_keys, const doubl
  * mask is NULL) and pred(a[i], threshold) holds; every comparison with a NaN `a`
  * fails, as in the reference's filter kernels.  Rows whose v is NaN are skipped by
  * every aggregate but, in the hash entry point, still create their key's group. */
-typedef enum { TBGB_F64 = 0, TBGB_F32 = 1 } tbgb_dtype;
+typedef enum {
+  TBGB_F64 = 0,
+  TBGB_F32 = 1,
+  TBGB_F16 = 2, /* rows of logits only (tbgb_logits, tbgb_teacher) */
+  TBGB_BF16 = 3
+} tbgb_dtype;
 typedef enum {
   TBGB_PRED_NONE = 0,    /* every row                 */
   TBGB_PRED_GT = 1,      /* a >  threshold            */
@@ -329,6 +334,97 @@ typedef struct {
 tbgb_status tbgb_fused_bin_stats(tbgb_ctx* ctx, const double* d_data, int64_t n_ticks, int32_t n_columns,
                                  const int64_t* d_boundaries, int64_t n_bins, const tbgb_bin_stats* out,
                                  void* stream);
+
+/* ---- rows of logits -----------------------------------------------------------------
+ * No counterpart in the reference: per-row reductions and selections over a vocabulary, for a
+ * table of a language model's logits (recording a teacher, training a student on the record,
+ * answering).  The reductions are those of the grouped statistics (a row is a contiguous bin),
+ * masks are this library's row masks, and sampled tokens are int32 codes for the dense groupby.
+ *
+ * A table of logits is `rows` rows of `vocab` elements (F32, F16 or BF16; 1 <= vocab <= 2^22),
+ * row r at data + r * row_stride elements (row_stride >= 0; rows that are only read may overlap,
+ * rows may start at any element).  rows == 0 is a call without work; rows <= 2^24.  Masks: bit i % 64 of word i / 64 allows token i, row r's words at
+ * d_mask + r * mask_stride (mask_stride 0: one mask for every row; NULL: everything is allowed). */
+typedef struct {
+  const void* data;
+  int64_t rows;
+  int64_t vocab;
+  int64_t row_stride;
+  int32_t dtype;
+  int32_t reserved;
+} tbgb_logits;
+
+/* The k largest logits of every row, by (logit descending, id ascending), 1 <= k <= 1024:
+ * values [rows][k] in the logits' type, ids [rows][k].  Logits that are NaN or -inf or not allowed
+ * are never taken; a row with fewer than k others ends in (-inf, -1).  lse [rows] (NULL to skip):
+ * log sum exp(z / temperature) over the allowed logits that are not NaN, -inf when there are none. */
+tbgb_status tbgb_top_logits(tbgb_ctx* ctx, const tbgb_logits* x, int32_t k, float temperature,
+                            const uint64_t* d_mask, int64_t mask_stride, void* d_values, int32_t* d_ids,
+                            float* d_lse, void* stream);
+
+/* A teacher's record: per row k entries (token id, logit); id -1 marks an unused entry; the ids of
+ * a row differ.  lse NULL: the teacher is the softmax of logits / temperature over the entries.
+ * lse [rows]: the teacher's log sum exp(logits / temperature) over its whole vocabulary; the entries
+ * then have p_i = exp(logit_i / temperature - lse), and "any other token" is one more outcome with
+ * the rest. */
+typedef struct {
+  const int32_t* ids;  /* row r at ids + r * ids_stride */
+  const void* logits;  /* row r at logits + r * logits_stride elements */
+  const float* lse;
+  int64_t ids_stride;
+  int64_t logits_stride;
+  int32_t dtype;       /* of logits: F32, F16 or BF16 */
+  int32_t k;           /* 1 <= k <= 1024 */
+  float temperature;   /* of teacher and student, > 0 */
+  int32_t reserved;
+} tbgb_teacher;
+
+/* KL divergence of the student q = softmax(z / temperature) from the teacher, per row (in nats):
+ *   loss[r]  = sum p_i (log p_i - log q_i)  [+ p_r (log p_r - log q_r), the other-token outcome;
+ *              left out where the student has no logit above -inf outside the entries]
+ *   stats[r] = (log sum exp(z / temperature), factor): what tbgb_distill_grad needs again
+ * A row without entries has loss 0.  NaN or +inf logits, and a row of nothing but -inf, make the
+ * row's loss and gradient NaN.  An id outside [-1, vocab) makes tbgb_sync report
+ * TBGB_ERR_KEY_OUT_OF_RANGE (the entry is left out), an id named twice in a row
+ * TBGB_ERR_INVALID_ARGUMENT (the row's outputs are then unspecified). */
+tbgb_status tbgb_distill_loss(tbgb_ctx* ctx, const tbgb_logits* x, const tbgb_teacher* teacher, float* d_loss,
+                              float* d_stats, void* stream);
+/* The gradient of sum_r weight[r] * loss[r] by the logits, in the logits' type (row r at grad +
+ * r * grad_stride elements; grad may be the logits' own memory with the same stride), from the
+ * stats of the loss on the same logits and teacher.  A row with weight 0 is padding: it is not
+ * read, its gradient is 0. */
+tbgb_status tbgb_distill_grad(tbgb_ctx* ctx, const tbgb_logits* x, const tbgb_teacher* teacher,
+                              const float* d_stats, const float* d_weight, void* d_grad, int64_t grad_stride,
+                              void* stream);
+/* Both in one pass over the logits, for weights known beforehand.  A row with weight 0 is padding: it
+ * is not read, its loss and gradient are 0 and its stats (0, 1). */
+tbgb_status tbgb_distill_step(tbgb_ctx* ctx, const tbgb_logits* x, const tbgb_teacher* teacher,
+                              const float* d_weight, float* d_loss, float* d_stats, void* d_grad,
+                              int64_t grad_stride, void* stream);
+
+/* How tokens are sampled: per row where the array is not NULL, else the same for every row. */
+typedef struct {
+  const float* temperature;
+  const int32_t* top_k;
+  const float* top_p;
+  const float* min_p;
+  float temperature_all; /* <= 0 (or NaN): the largest logit, lowest id first */
+  int32_t top_k_all;     /* <= 0: off */
+  float top_p_all;       /* >= 1: off */
+  float min_p_all;       /* <= 0: off */
+} tbgb_sampling;
+
+/* One token per row from the uniform numbers u [rows] in [0, 1).  A token's weight is
+ * 2^((z - zmax) * (log2(e) / temperature)) in 32 bits, rounded to a multiple of 2^-30, so that sums
+ * of weights are exact and a token does not depend on their order.  top-k keeps the first k by (logit
+ * descending, id ascending); top-p of those, with sum W, the shortest prefix that reaches ceil(p W);
+ * min-p of those the tokens whose weight before rounding is at least min_p.  The token is the first, in
+ * the order of the ids, whose running sum exceeds floor(u W'), W' the sum of what is kept.
+ * logprobs (NULL to skip): the log of the token's share of W'.  NaN, -inf and masked logits are
+ * never taken; a row without any other gets token -1 and logprob -inf. */
+tbgb_status tbgb_sample_tokens(tbgb_ctx* ctx, const tbgb_logits* x, const float* d_u, const tbgb_sampling* p,
+                               const uint64_t* d_mask, int64_t mask_stride, int32_t* d_tokens, float* d_logprobs,
+                               void* stream);
 
 /* ---- sharded dense groupby over NVLink peer memory (one process per GPU) ----------------
  * The exchange step without a library collective: every rank owns an exchange buffer

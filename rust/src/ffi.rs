@@ -55,6 +55,8 @@ impl Default for tbgb_moments {
 
 pub const TBGB_F64: i32 = 0;
 pub const TBGB_F32: i32 = 1;
+pub const TBGB_F16: i32 = 2;
+pub const TBGB_BF16: i32 = 3;
 
 pub const TBGB_PRED_NONE: i32 = 0;
 pub const TBGB_PRED_GT: i32 = 1;
@@ -142,6 +144,47 @@ pub struct tbgb_bin_stats {
     pub std: *mut f64,
 }
 
+/// A table of logits: `rows` rows of `vocab` elements (F32, F16 or BF16).
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct tbgb_logits {
+    pub data: *const c_void,
+    pub rows: i64,
+    pub vocab: i64,
+    pub row_stride: i64,
+    pub dtype: i32,
+    pub reserved: i32,
+}
+
+/// A teacher's recorded top logits (`lse` null: closed among the entries).
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct tbgb_teacher {
+    pub ids: *const i32,
+    pub logits: *const c_void,
+    pub lse: *const f32,
+    pub ids_stride: i64,
+    pub logits_stride: i64,
+    pub dtype: i32,
+    pub k: i32,
+    pub temperature: f32,
+    pub reserved: i32,
+}
+
+/// Sampling parameters: per row where the array is not null, else the same for every row.
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct tbgb_sampling {
+    pub temperature: *const f32,
+    pub top_k: *const i32,
+    pub top_p: *const f32,
+    pub min_p: *const f32,
+    pub temperature_all: f32,
+    pub top_k_all: i32,
+    pub top_p_all: f32,
+    pub min_p_all: f32,
+}
+
 extern "C" {
     // ---- context -----------------------------------------------------------------------
     pub fn tbgb_create(device: c_int, out: *mut *mut tbgb_ctx) -> tbgb_status;
@@ -214,6 +257,22 @@ extern "C" {
     pub fn tbgb_fused_bin_stats(ctx: *mut tbgb_ctx, data: *const f64, n_ticks: i64, n_columns: i32,
                                 boundaries: *const i64, n_bins: i64, out: *const tbgb_bin_stats,
                                 stream: *mut c_void) -> tbgb_status;
+
+    // ---- rows of logits ---------------------------------------------------------------------
+    pub fn tbgb_top_logits(ctx: *mut tbgb_ctx, x: *const tbgb_logits, k: i32, temperature: f32, mask: *const u64,
+                           mask_stride: i64, values: *mut c_void, ids: *mut i32, lse: *mut f32,
+                           stream: *mut c_void) -> tbgb_status;
+    pub fn tbgb_distill_loss(ctx: *mut tbgb_ctx, x: *const tbgb_logits, teacher: *const tbgb_teacher,
+                             loss: *mut f32, stats: *mut f32, stream: *mut c_void) -> tbgb_status;
+    pub fn tbgb_distill_grad(ctx: *mut tbgb_ctx, x: *const tbgb_logits, teacher: *const tbgb_teacher,
+                             stats: *const f32, weight: *const f32, grad: *mut c_void, grad_stride: i64,
+                             stream: *mut c_void) -> tbgb_status;
+    pub fn tbgb_distill_step(ctx: *mut tbgb_ctx, x: *const tbgb_logits, teacher: *const tbgb_teacher,
+                             weight: *const f32, loss: *mut f32, stats: *mut f32, grad: *mut c_void,
+                             grad_stride: i64, stream: *mut c_void) -> tbgb_status;
+    pub fn tbgb_sample_tokens(ctx: *mut tbgb_ctx, x: *const tbgb_logits, u: *const f32, p: *const tbgb_sampling,
+                              mask: *const u64, mask_stride: i64, tokens: *mut i32, logprobs: *mut f32,
+                              stream: *mut c_void) -> tbgb_status;
 
     // ---- row shards: states, peer-memory exchange, owner routing -------------------------
     pub fn tbgb_state_bytes(n_groups: i32) -> usize;

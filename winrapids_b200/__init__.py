@@ -10,6 +10,7 @@ Two layers:
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import math
 from dataclasses import dataclass
@@ -18,14 +19,15 @@ import numpy as np
 
 from ._lib import (BIN_STATS_FIELDS, DTYPES, EXPRS, HIGHER_FIELDS, MOMENT_FIELDS, PREDS, TILE_STATS_BYTES,
                    TILE_STATS_FIELDS, BinStats, Columns,
-                   EntryNotFound, InvalidArgument, KeyOutOfRange, Moments, TableFull, TambearGbError, error_for, lib)
+                   EntryNotFound, InvalidArgument, KeyOutOfRange, Logits, Moments, Sampling, TableFull, TambearGbError,
+                   Teacher, error_for, lib)
 
 __all__ = [
     "ComputeEngine", "AccumulateEngine", "HashScatterEngine", "GroupByResult", "Grouping", "Op", "GroupIndex",
     "Context", "DescriptiveEngine", "GroupedMomentStats", "MomentStats", "TambearGbError", "KeyOutOfRange",
     "InvalidArgument", "TableFull", "EntryNotFound", "MOMENT_FIELDS", "HIGHER_FIELDS", "SUMCOUNT_FIELDS",
     "FilterJit", "MaskOp", "Frame", "GroupByBuilder", "from_columns", "fused_bin_stats",
-    "fused_multi_column_bin_stats",
+    "fused_multi_column_bin_stats", "TopLogits", "top_logits", "distill_loss", "sample_tokens",
 ]
 
 SUMCOUNT_FIELDS = ("count", "sum", "mean")
@@ -314,6 +316,203 @@ class Context:
         self._check(self._L.tbgb_mask_skip_tiles(self._h, _ptr(mask), _ptr(skip), int(tile_rows), int(n_rows),
                                                  _ptr(m), _stream_handle(stream)))
         return m
+
+    # ---- rows of logits: a teacher's top logits, distillation, sampling ----
+    # Logits are an f32, f16 or bf16 device tensor [rows, vocab] whose rows may lie anywhere (any row
+    # stride, any alignment); token masks are row masks of the vocabulary, int64 [words] for every row
+    # or [rows, words].
+
+    def _stream_scope(self, stream, *tensors):
+        """The handle of `stream` (None: torch's current one) and a scope in which new tensors belong to
+        it.  Tensors that come from another stream are kept until the work on `stream` is done."""
+        torch = _torch()
+        if stream is None:
+            return torch.cuda.current_stream(self.device).cuda_stream, contextlib.nullcontext()
+        if not isinstance(stream, torch.cuda.Stream):
+            stream = torch.cuda.ExternalStream(_stream_handle(stream), device=self.device)
+        for t in tensors:
+            if t is not None:
+                t.record_stream(stream)
+        return stream.cuda_stream, torch.cuda.stream(stream)
+
+    def _tensor(self, t, what: str, dtypes, shape=None):
+        torch = _torch()
+        if not isinstance(t, torch.Tensor) or not t.is_cuda or t.device.index != self.device:
+            raise InvalidArgument(7, f"{what} must be a tensor on cuda:{self.device}")
+        if t.dtype not in dtypes:
+            raise InvalidArgument(7, f"{what} has dtype {t.dtype}, not one of {', '.join(map(str, dtypes))}")
+        if shape is not None and tuple(t.shape) != tuple(shape):
+            raise InvalidArgument(7, f"{what} has shape {tuple(t.shape)}, not {tuple(shape)}")
+        return t
+
+    def _rows_tensor(self, t, what: str, dtypes, shape=None):
+        """A 2-d tensor whose rows are contiguous, with the stride from one row to the next."""
+        self._tensor(t, what, dtypes, shape)
+        if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+            raise InvalidArgument(7, f"{what} must be a 2-d tensor with contiguous rows")
+        return t, int(t.stride(0)) if t.shape[0] > 1 else int(t.shape[1])
+
+    def _row_vector(self, t, what: str, dtype, rows: int, cols: int | None = None):
+        self._tensor(t, what, (dtype,), (rows,) if cols is None else (rows, cols))
+        if not t.is_contiguous():
+            raise InvalidArgument(7, f"{what} must be contiguous")
+        return t
+
+    def _out(self, out, name: str, dtype, shape):
+        torch = _torch()
+        t = (out or {}).get(name)
+        if t is None:
+            return torch.empty(shape, dtype=dtype, device=f"cuda:{self.device}")
+        self._tensor(t, name, (dtype,), shape)
+        if not t.is_contiguous():
+            raise InvalidArgument(7, f"{name} must be contiguous")
+        return t
+
+    def _logits(self, logits) -> Logits:
+        torch = _torch()
+        codes = {torch.float32: "f32", torch.float16: "f16", torch.bfloat16: "bf16"}
+        t, ld = self._rows_tensor(logits, "logits", tuple(codes))
+        return Logits(_ptr(t), int(t.shape[0]), int(t.shape[1]), ld, DTYPES[codes[t.dtype]], 0)
+
+    def _token_mask(self, mask, x: Logits):
+        torch = _torch()
+        if mask is None:
+            return None, 0
+        words = (x.vocab + 63) // 64
+        if mask.dim() == 1:
+            self._tensor(mask, "mask", (torch.int64,), (words,))
+            if words > 1 and mask.stride(0) != 1:
+                raise InvalidArgument(7, "mask must be contiguous")
+            return mask, 0
+        t, ld = self._rows_tensor(mask, "mask", (torch.int64,), (x.rows, words))
+        return t, ld
+
+    def top_logits(self, logits, k: int, temperature: float = 1.0, mask=None, lse: bool = True,
+                   out: dict | None = None, stream=None, sync: bool = True) -> dict:
+        """The k largest logits of every row by (logit descending, id ascending): values [rows, k] in
+        the logits' dtype, ids int32 [rows, k], and with lse the rows' log sum exp(z / temperature)
+        (tbgb_top_logits).  NaN, -inf and masked logits are never taken; short rows end in (-inf, -1)."""
+        torch = _torch()
+        x = self._logits(logits)
+        m, mld = self._token_mask(mask, x)
+        if not 1 <= int(k) <= 1024:
+            raise InvalidArgument(7, "k must be in [1, 1024]")
+        handle, scope = self._stream_scope(stream, logits, m, *(out or {}).values())
+        with scope:
+            res = {"values": self._out(out, "values", logits.dtype, (x.rows, int(k))),
+                   "ids": self._out(out, "ids", torch.int32, (x.rows, int(k)))}
+            if lse:
+                res["lse"] = self._out(out, "lse", torch.float32, (x.rows,))
+        self._check(self._L.tbgb_top_logits(self._h, C.byref(x), int(k), float(temperature), _ptr(m), mld,
+                                            _ptr(res["values"]), _ptr(res["ids"]), _ptr(res.get("lse")), handle))
+        if sync:
+            self.sync(handle)
+        return res
+
+    def _teacher(self, x: Logits, ids, teacher, teacher_lse, temperature) -> Teacher:
+        torch = _torch()
+        codes = {torch.float32: "f32", torch.float16: "f16", torch.bfloat16: "bf16"}
+        ids, ids_ld = self._rows_tensor(ids, "ids", (torch.int32,))
+        t, ld = self._rows_tensor(teacher, "teacher", tuple(codes), (x.rows, int(ids.shape[1])))
+        if int(ids.shape[0]) != x.rows:
+            raise InvalidArgument(7, "ids and logits must have the same number of rows")
+        if teacher_lse is not None:
+            self._row_vector(teacher_lse, "teacher_lse", torch.float32, x.rows)
+        return Teacher(_ptr(ids), _ptr(t), _ptr(teacher_lse), ids_ld, ld, DTYPES[codes[t.dtype]], int(ids.shape[1]),
+                       float(temperature), 0)
+
+    def _gradient(self, grad, logits):
+        torch = _torch()
+        if grad is None:
+            grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        return self._rows_tensor(grad, "grad", (logits.dtype,), logits.shape)
+
+    def distill_loss(self, logits, ids, teacher, teacher_lse=None, temperature: float = 1.0,
+                     out: dict | None = None, stream=None, sync: bool = True) -> dict:
+        """Per row, the KL divergence of softmax(logits / temperature) from a teacher recorded as ids
+        (int32 [rows, k], -1: unused) and teacher (its logits there): loss f32 [rows] and the stats
+        [rows, 2] that distill_grad takes (tbgb_distill_loss).  With teacher_lse [rows] the teacher's
+        remaining probability is one more outcome; without it the teacher is closed among its entries."""
+        torch = _torch()
+        x = self._logits(logits)
+        t = self._teacher(x, ids, teacher, teacher_lse, temperature)
+        handle, scope = self._stream_scope(stream, logits, ids, teacher, teacher_lse, *(out or {}).values())
+        with scope:
+            res = {"loss": self._out(out, "loss", torch.float32, (x.rows,)),
+                   "stats": self._out(out, "stats", torch.float32, (x.rows, 2))}
+        self._check(self._L.tbgb_distill_loss(self._h, C.byref(x), C.byref(t), _ptr(res["loss"]), _ptr(res["stats"]),
+                                              handle))
+        if sync:
+            self.sync(handle)
+        return res
+
+    def distill_grad(self, logits, ids, teacher, stats, weight, teacher_lse=None, temperature: float = 1.0, grad=None,
+                     stream=None, sync: bool = True):
+        """The gradient of sum(weight * loss) by the logits, from the stats of distill_loss on the same
+        arguments (tbgb_distill_grad); weight f32 [rows].  `grad` may be `logits` itself."""
+        torch = _torch()
+        x = self._logits(logits)
+        t = self._teacher(x, ids, teacher, teacher_lse, temperature)
+        self._row_vector(stats, "stats", torch.float32, x.rows, 2)
+        self._row_vector(weight, "weight", torch.float32, x.rows)
+        handle, scope = self._stream_scope(stream, logits, ids, teacher, teacher_lse, stats, weight, grad)
+        with scope:
+            g, ld = self._gradient(grad, logits)
+        self._check(self._L.tbgb_distill_grad(self._h, C.byref(x), C.byref(t), _ptr(stats), _ptr(weight), _ptr(g), ld,
+                                              handle))
+        if sync:
+            self.sync(handle)
+        return g
+
+    def distill_step(self, logits, ids, teacher, weight, teacher_lse=None, temperature: float = 1.0, grad=None,
+                     out: dict | None = None, stream=None, sync: bool = True) -> dict:
+        """distill_loss and distill_grad in one pass over the logits (tbgb_distill_step): loss, stats and
+        grad.  A row with weight 0 is padding: it is not read, its loss and gradient are 0."""
+        torch = _torch()
+        x = self._logits(logits)
+        t = self._teacher(x, ids, teacher, teacher_lse, temperature)
+        self._row_vector(weight, "weight", torch.float32, x.rows)
+        handle, scope = self._stream_scope(stream, logits, ids, teacher, teacher_lse, weight, grad,
+                                           *(out or {}).values())
+        with scope:
+            g, ld = self._gradient(grad, logits)
+            res = {"loss": self._out(out, "loss", torch.float32, (x.rows,)),
+                   "stats": self._out(out, "stats", torch.float32, (x.rows, 2)), "grad": g}
+        self._check(self._L.tbgb_distill_step(self._h, C.byref(x), C.byref(t), _ptr(weight), _ptr(res["loss"]),
+                                              _ptr(res["stats"]), _ptr(g), ld, handle))
+        if sync:
+            self.sync(handle)
+        return res
+
+    def sample_tokens(self, logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, mask=None, logprobs: bool = True,
+                      out: dict | None = None, stream=None, sync: bool = True) -> dict:
+        """One token per row from the uniform numbers u (f32 [rows], in [0, 1)): tokens int32 [rows] and
+        logprobs f32 [rows] (tbgb_sample_tokens).  temperature, top_p and min_p are numbers or f32 tensors
+        [rows], top_k a number or an int32 tensor; temperature <= 0 takes the largest logit, top_k <= 0,
+        top_p >= 1 and min_p <= 0 are off.  A row without any token to take gets -1 and -inf."""
+        torch = _torch()
+        x = self._logits(logits)
+        self._row_vector(u, "u", torch.float32, x.rows)
+        m, mld = self._token_mask(mask, x)
+        p = Sampling()
+        kept = []
+        for name, value, dtype in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
+                                   ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
+            if isinstance(value, torch.Tensor):
+                kept.append(self._row_vector(value, name, dtype, x.rows))
+                setattr(p, name, _ptr(value))
+            else:
+                setattr(p, name + "_all", int(value) if name == "top_k" else float(value))
+        handle, scope = self._stream_scope(stream, logits, u, m, *kept, *(out or {}).values())
+        with scope:
+            res = {"tokens": self._out(out, "tokens", torch.int32, (x.rows,))}
+            if logprobs:
+                res["logprobs"] = self._out(out, "logprobs", torch.float32, (x.rows,))
+        self._check(self._L.tbgb_sample_tokens(self._h, C.byref(x), _ptr(u), C.byref(p), _ptr(m), mld,
+                                               _ptr(res["tokens"]), _ptr(res.get("logprobs")), handle))
+        if sync:
+            self.sync(handle)
+        return res
 
     def groupby_hash_into(self, keys, a, max_groups: int, out_keys, out: dict, n_groups, b=None, c=None,
                           expr: str = "a", pred: str | None = None, threshold: float = 0.0, mask=None,
@@ -657,3 +856,4 @@ from .engines import AccumulateEngine, ComputeEngine, GroupByResult, Grouping, H
 from .group_index import GroupIndex  # noqa: E402
 from .frame import FilterJit, Frame, GroupByBuilder, MaskOp, from_columns  # noqa: E402
 from .bins import fused_bin_stats, fused_multi_column_bin_stats  # noqa: E402
+from .logits import TopLogits, distill_loss, sample_tokens, top_logits  # noqa: E402

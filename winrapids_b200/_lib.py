@@ -69,9 +69,32 @@ class Columns(C.Structure):
                 ("expr", C.c_int32), ("pred", C.c_int32), ("reserved", C.c_int32), ("threshold", C.c_double)]
 
 
-DTYPES = {"f64": 0, "f32": 1}
+DTYPES = {"f64": 0, "f32": 1, "f16": 2, "bf16": 3}
 PREDS = {None: 0, "none": 0, ">": 1, ">=": 2, "<": 3, "<=": 4, "not_nan": 5, "finite": 6}
 EXPRS = {"a": 0, "a+b": 1, "a-b": 2, "a*b": 3, "a*b+1": 4, "a*b+c": 5}
+
+
+class Logits(C.Structure):
+    """tbgb_logits: a table of logits (rows of a vocabulary)."""
+
+    _fields_ = [("data", C.c_void_p), ("rows", C.c_int64), ("vocab", C.c_int64), ("row_stride", C.c_int64),
+                ("dtype", C.c_int32), ("reserved", C.c_int32)]
+
+
+class Teacher(C.Structure):
+    """tbgb_teacher: a teacher's recorded top logits."""
+
+    _fields_ = [("ids", C.c_void_p), ("logits", C.c_void_p), ("lse", C.c_void_p), ("ids_stride", C.c_int64),
+                ("logits_stride", C.c_int64), ("dtype", C.c_int32), ("k", C.c_int32), ("temperature", C.c_float),
+                ("reserved", C.c_int32)]
+
+
+class Sampling(C.Structure):
+    """tbgb_sampling: per-row arrays, or one value for every row where the array is NULL."""
+
+    _fields_ = [("temperature", C.c_void_p), ("top_k", C.c_void_p), ("top_p", C.c_void_p), ("min_p", C.c_void_p),
+                ("temperature_all", C.c_float), ("top_k_all", C.c_int32), ("top_p_all", C.c_float),
+                ("min_p_all", C.c_float)]
 
 
 class Moments(C.Structure):
@@ -137,6 +160,11 @@ def lib() -> C.CDLL:
         "tbgb_tile_skip_mask": (st, [vp, vp, i64, i32, f64, vp, vp]),
         "tbgb_mask_skip_tiles": (st, [vp, vp, vp, i64, i64, vp, vp]),
         "tbgb_fused_bin_stats": (st, [vp, vp, i64, i32, vp, i64, vp, vp]),
+        "tbgb_top_logits": (st, [vp, C.POINTER(Logits), i32, C.c_float, vp, i64, vp, vp, vp, vp]),
+        "tbgb_distill_loss": (st, [vp, C.POINTER(Logits), C.POINTER(Teacher), vp, vp, vp]),
+        "tbgb_distill_grad": (st, [vp, C.POINTER(Logits), C.POINTER(Teacher), vp, vp, vp, i64, vp]),
+        "tbgb_distill_step": (st, [vp, C.POINTER(Logits), C.POINTER(Teacher), vp, vp, vp, vp, i64, vp]),
+        "tbgb_sample_tokens": (st, [vp, C.POINTER(Logits), vp, C.POINTER(Sampling), vp, i64, vp, vp, vp]),
         "tbgb_exchange_bytes": (C.c_size_t, [i32, i32]),
         "tbgb_exchange_alloc": (st, [vp, i32, i32, C.POINTER(vp)]),
         "tbgb_exchange_free": (st, [vp, vp]),
@@ -177,6 +205,7 @@ HEADER_SYMBOLS = (
     "tbgb_exchange_bytes", "tbgb_exchange_alloc", "tbgb_exchange_free", "tbgb_peer_export", "tbgb_peer_import",
     "tbgb_peer_close", "tbgb_groupby_dense_sharded", "tbgb_radix_value_bytes", "tbgb_radix_route",
     "tbgb_radix_groupby_routed", "tbgb_radix_fallback", "tbgb_ipc_alloc", "tbgb_ipc_free",
+    "tbgb_top_logits", "tbgb_distill_loss", "tbgb_distill_grad", "tbgb_distill_step", "tbgb_sample_tokens",
 )
 
 # tbgb_bin_stats field order

@@ -14,6 +14,7 @@
 #include "errbits.hpp"
 #include "gen.cuh"
 #include "group_index.cuh"
+#include "logits.cuh"
 #include "mask.cuh"
 #include "partition.cuh"
 #include "phi.cuh"
@@ -886,6 +887,196 @@ tbgb_status tbgb_fused_bin_stats(tbgb_ctx* ctx, const double* d_data, int64_t n_
   return TBGB_OK;
 }
 
+// ---- rows of logits ----
+
+namespace {
+
+size_t elem_bytes(int32_t dtype) { return dtype == TBGB_F32 ? 4 : 2; }
+
+bool logit_dtype(int32_t d) { return d == TBGB_F32 || d == TBGB_F16 || d == TBGB_BF16; }
+
+tbgb_status check_logits(tbgb_ctx* ctx, const tbgb_logits* x, tbgb::LogitsArgs* out) {
+  if (!ctx) return TBGB_ERR_INVALID_ARGUMENT;
+  if (!x) return fail(ctx, TBGB_ERR_INVALID_ARGUMENT, "logits descriptor is NULL");
+  if (!logit_dtype(x->dtype)) return fail(ctx, TBGB_ERR_INVALID_ARGUMENT, "logits must be F32, F16 or BF16");
+  if (x->rows < 0 || x->rows > tbgb::kLogitRowsMax)
+    return fail(ctx, TBGB_ERR_INVALID_ARGUMENT, "rows must be in [0, 2^24]");
+  if (x->vocab < 1 || x->vocab > tbgb::kVocabMax)
+    return fail(ctx, TBGB_ERR_INVALID_ARGUMENT, "vocab must be in [1, 2^22]");
+  if (x->row_stride < 0) return fail(ctx, TBGB_ERR_INVALID_ARGUMENT, "row_stride must be >= 0");
+  if (x->rows > 0 && !x->data) return fail(ctx, TBGB_ERR_INVALID_ARGUMENT, "logits pointer is NULL");
+  if (misaligned(x->data, elem_bytes(x->dtype)))
+    return fail(ctx, TBGB_ERR_INVALID_ARGUMENT, "logits not aligned to their element size");
+  *out = tbgb::LogitsArgs{x->data, x->dtype, x->row_stride, x->rows, static_cast<int>(x->vocab)};
+  return TBGB_OK;
+}
+
+tbgb_status check_row_mask(tbgb_ctx* ctx, const tbgb_logits* x, const uint64_t* mask, int64_t stride) {
+  if (misaligned(mask, 8)) return fail(ctx, TBGB_ERR_INVALID_ARGUMENT, "mask is not 8-byte aligned");
+  if (mask && stride != 0 && stride < (x->vocab + 63) / 64)
+    return fail(ctx, TBGB_ERR_INVALID_ARGUMENT, "mask_stride must be 0 or at least ceil(vocab / 64) words");
+  return TBGB_OK;
+}
+
+// `n` floats (or int32s) per row that must be there when rows > 0
+tbgb_status check_row_array(tbgb_ctx* ctx, const void* p, int64_t rows, const char* what) {
+  if (rows > 0 && !p) return fail(ctx, TBGB_ERR_INVALID_ARGUMENT, std::string(what) + " is NULL");
+  if (misaligned(p, 4)) return fail(ctx, TBGB_ERR_INVALID_ARGUMENT, std::string(what) + " is not 4-byte aligned");
+  return TBGB_OK;
+}
+
+// not a finite number above zero
+bool bad_temperature(float t) { return !(t > 0.0f) || t > 3.4028234e38f; }
+
+tbgb_status check_teacher(tbgb_ctx* ctx, const tbgb_logits* x, const tbgb_teacher* t, tbgb::DistillArgs* a) {
+  tbgb_status st = check_logits(ctx, x, &a->x);
+  if (st != TBGB_OK) return st;
+  if (!t) return fail(ctx, TBGB_ERR_INVALID_ARGUMENT, "teacher descriptor is NULL");
+  if (!logit_dtype(t->dtype)) return fail(ctx, TBGB_ERR_INVALID_ARGUMENT, "teacher logits must be F32, F16 or BF16");
+  if (t->k < 1 || t->k > tbgb::kTopMax) return fail(ctx, TBGB_ERR_INVALID_ARGUMENT, "k must be in [1, 1024]");
+  if (t->ids_stride < 0 || t->logits_stride < 0)
+    return fail(ctx, TBGB_ERR_INVALID_ARGUMENT, "the record's strides must be >= 0");
+  if (bad_temperature(t->temperature))
+    return fail(ctx, TBGB_ERR_INVALID_ARGUMENT, "temperature must be positive and finite");
+  if (misaligned(t->lse, 4)) return fail(ctx, TBGB_ERR_INVALID_ARGUMENT, "teacher lse is not 4-byte aligned");
+  st = check_row_array(ctx, t->ids, x->rows, "teacher ids");
+  if (st != TBGB_OK) return st;
+  if (x->rows > 0 && !t->logits) return fail(ctx, TBGB_ERR_INVALID_ARGUMENT, "teacher logits is NULL");
+  if (misaligned(t->logits, elem_bytes(t->dtype)))
+    return fail(ctx, TBGB_ERR_INVALID_ARGUMENT, "teacher logits not aligned to their element size");
+  a->ids = t->ids;
+  a->ids_ld = t->ids_stride;
+  a->teacher = t->logits;
+  a->teacher_dtype = t->dtype;
+  a->teacher_ld = t->logits_stride;
+  a->k = t->k;
+  a->teacher_lse = t->lse;
+  a->temperature = t->temperature;
+  a->err = ctx->err;
+  return TBGB_OK;
+}
+
+tbgb_status check_grad(tbgb_ctx* ctx, const tbgb_logits* x, void* grad, int64_t stride) {
+  if (x->rows > 0 && !grad) return fail(ctx, TBGB_ERR_INVALID_ARGUMENT, "grad is NULL");
+  if (misaligned(grad, elem_bytes(x->dtype)))
+    return fail(ctx, TBGB_ERR_INVALID_ARGUMENT, "grad not aligned to its element size");
+  if (stride < 0 || (x->rows > 1 && stride < x->vocab))
+    return fail(ctx, TBGB_ERR_INVALID_ARGUMENT, "rows of the gradient overlap (grad_stride < vocab)");
+  return TBGB_OK;
+}
+
+tbgb_status run_distill(tbgb_ctx* ctx, const tbgb::DistillArgs& a, bool with_loss, bool with_grad, void* stream) {
+  DeviceGuard dg(ctx->device);
+  if (!dg.ok) return fail(ctx, TBGB_ERR_BACKEND, "cudaSetDevice failed");
+  cudaError_t e = tbgb::distill_launch(a, with_loss, with_grad, ctx->num_sms, static_cast<cudaStream_t>(stream),
+                                       &ctx->launches);
+  if (e != cudaSuccess) return cuda_fail(ctx, TBGB_ERR_DISPATCH, "distillation launch", e);
+  return TBGB_OK;
+}
+
+}  // namespace
+
+tbgb_status tbgb_top_logits(tbgb_ctx* ctx, const tbgb_logits* x, int32_t k, float temperature,
+                            const uint64_t* d_mask, int64_t mask_stride, void* d_values, int32_t* d_ids,
+                            float* d_lse, void* stream) {
+  tbgb::TopArgs a{};
+  tbgb_status st = check_logits(ctx, x, &a.x);
+  if (st == TBGB_OK) st = check_row_mask(ctx, x, d_mask, mask_stride);
+  if (st == TBGB_OK) st = check_row_array(ctx, d_ids, x->rows, "ids");
+  if (st != TBGB_OK) return st;
+  if (k < 1 || k > tbgb::kTopMax) return fail(ctx, TBGB_ERR_INVALID_ARGUMENT, "k must be in [1, 1024]");
+  if (bad_temperature(temperature))
+    return fail(ctx, TBGB_ERR_INVALID_ARGUMENT, "temperature must be positive and finite");
+  if (x->rows > 0 && !d_values) return fail(ctx, TBGB_ERR_INVALID_ARGUMENT, "values is NULL");
+  if (misaligned(d_values, elem_bytes(x->dtype)) || misaligned(d_lse, 4))
+    return fail(ctx, TBGB_ERR_INVALID_ARGUMENT, "an output is not aligned to its element size");
+  a.k = k;
+  a.temperature = temperature;
+  a.mask = d_mask;
+  a.mask_ld = mask_stride;
+  a.values = d_values;
+  a.ids = d_ids;
+  a.lse = d_lse;
+  DeviceGuard dg(ctx->device);
+  if (!dg.ok) return fail(ctx, TBGB_ERR_BACKEND, "cudaSetDevice failed");
+  cudaError_t e = tbgb::top_logits_launch(a, ctx->num_sms, static_cast<cudaStream_t>(stream), &ctx->launches);
+  if (e != cudaSuccess) return cuda_fail(ctx, TBGB_ERR_DISPATCH, "top logits launch", e);
+  return TBGB_OK;
+}
+
+tbgb_status tbgb_distill_loss(tbgb_ctx* ctx, const tbgb_logits* x, const tbgb_teacher* teacher, float* d_loss,
+                              float* d_stats, void* stream) {
+  tbgb::DistillArgs a{};
+  tbgb_status st = check_teacher(ctx, x, teacher, &a);
+  if (st == TBGB_OK) st = check_row_array(ctx, d_loss, x->rows, "loss");
+  if (st == TBGB_OK) st = check_row_array(ctx, d_stats, x->rows, "stats");
+  if (st != TBGB_OK) return st;
+  a.loss = d_loss;
+  a.stats = d_stats;
+  return run_distill(ctx, a, true, false, stream);
+}
+
+tbgb_status tbgb_distill_grad(tbgb_ctx* ctx, const tbgb_logits* x, const tbgb_teacher* teacher,
+                              const float* d_stats, const float* d_weight, void* d_grad, int64_t grad_stride,
+                              void* stream) {
+  tbgb::DistillArgs a{};
+  tbgb_status st = check_teacher(ctx, x, teacher, &a);
+  if (st == TBGB_OK) st = check_row_array(ctx, d_stats, x->rows, "stats");
+  if (st == TBGB_OK) st = check_row_array(ctx, d_weight, x->rows, "weight");
+  if (st == TBGB_OK) st = check_grad(ctx, x, d_grad, grad_stride);
+  if (st != TBGB_OK) return st;
+  a.stats = const_cast<float*>(d_stats);
+  a.weight = d_weight;
+  a.grad = d_grad;
+  a.grad_ld = grad_stride;
+  return run_distill(ctx, a, false, true, stream);
+}
+
+tbgb_status tbgb_distill_step(tbgb_ctx* ctx, const tbgb_logits* x, const tbgb_teacher* teacher,
+                              const float* d_weight, float* d_loss, float* d_stats, void* d_grad,
+                              int64_t grad_stride, void* stream) {
+  tbgb::DistillArgs a{};
+  tbgb_status st = check_teacher(ctx, x, teacher, &a);
+  if (st == TBGB_OK) st = check_row_array(ctx, d_weight, x->rows, "weight");
+  if (st == TBGB_OK) st = check_row_array(ctx, d_loss, x->rows, "loss");
+  if (st == TBGB_OK) st = check_row_array(ctx, d_stats, x->rows, "stats");
+  if (st == TBGB_OK) st = check_grad(ctx, x, d_grad, grad_stride);
+  if (st != TBGB_OK) return st;
+  a.weight = d_weight;
+  a.loss = d_loss;
+  a.stats = d_stats;
+  a.grad = d_grad;
+  a.grad_ld = grad_stride;
+  return run_distill(ctx, a, true, true, stream);
+}
+
+tbgb_status tbgb_sample_tokens(tbgb_ctx* ctx, const tbgb_logits* x, const float* d_u, const tbgb_sampling* p,
+                               const uint64_t* d_mask, int64_t mask_stride, int32_t* d_tokens, float* d_logprobs,
+                               void* stream) {
+  tbgb::SampleArgs a{};
+  tbgb_status st = check_logits(ctx, x, &a.x);
+  if (st != TBGB_OK) return st;
+  if (!p) return fail(ctx, TBGB_ERR_INVALID_ARGUMENT, "sampling parameters are NULL");
+  st = check_row_mask(ctx, x, d_mask, mask_stride);
+  if (st == TBGB_OK) st = check_row_array(ctx, d_u, x->rows, "u");
+  if (st == TBGB_OK) st = check_row_array(ctx, d_tokens, x->rows, "tokens");
+  if (st != TBGB_OK) return st;
+  const void* ptrs[] = {p->temperature, p->top_k, p->top_p, p->min_p, d_logprobs};
+  for (const void* q : ptrs)
+    if (misaligned(q, 4)) return fail(ctx, TBGB_ERR_INVALID_ARGUMENT, "a per-row array is not 4-byte aligned");
+  a.u = d_u;
+  a.p = *p;
+  a.mask = d_mask;
+  a.mask_ld = mask_stride;
+  a.tokens = d_tokens;
+  a.logprobs = d_logprobs;
+  DeviceGuard dg(ctx->device);
+  if (!dg.ok) return fail(ctx, TBGB_ERR_BACKEND, "cudaSetDevice failed");
+  cudaError_t e = tbgb::sample_launch(a, ctx->num_sms, static_cast<cudaStream_t>(stream), &ctx->launches);
+  if (e != cudaSuccess) return cuda_fail(ctx, TBGB_ERR_DISPATCH, "sampling launch", e);
+  return TBGB_OK;
+}
+
 // ---- row masks and tile statistics ----
 
 namespace {
@@ -1224,6 +1415,10 @@ tbgb_status tbgb_sync(tbgb_ctx* ctx, void* stream) {
   if (bits & tbgb::KERR_TIMEOUT) return fail(ctx, TBGB_ERR_TIMEOUT, "device-side wait timed out");
   if (bits & tbgb::KERR_BOUNDARIES)
     return fail(ctx, TBGB_ERR_INVALID_ARGUMENT, "bin boundaries are not non-decreasing within [0, n_ticks]");
+  if (bits & tbgb::KERR_TOKEN_ID)
+    return fail(ctx, TBGB_ERR_KEY_OUT_OF_RANGE, "a teacher's token id is outside [-1, vocab)");
+  if (bits & tbgb::KERR_TOKEN_TWICE)
+    return fail(ctx, TBGB_ERR_INVALID_ARGUMENT, "a row of the teacher's record names a token twice");
   if (bits & tbgb::KERR_MISALIGNED) return fail(ctx, TBGB_ERR_INVALID_ARGUMENT, "a staged column is not 16-byte aligned");
   return fail(ctx, TBGB_ERR_BACKEND, "unknown device error bits " + std::to_string(bits));
 }

@@ -12,6 +12,8 @@ enum : uint32_t {
   KERR_TABLE_FULL = 1u << 2,  // hash table probe limit reached
   KERR_MISALIGNED = 1u << 3,  // staged copy source not 16-byte aligned
   KERR_BOUNDARIES = 1u << 4,  // bin boundaries not non-decreasing within [0, n_ticks]
+  KERR_TOKEN_ID = 1u << 5,    // a teacher's token id outside [-1, vocabulary)
+  KERR_TOKEN_TWICE = 1u << 6, // a row of a teacher's record names a token twice
 };
 
 }  // namespace tbgb

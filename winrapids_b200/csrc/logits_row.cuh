@@ -1,0 +1,330 @@
+// logits_row.cuh -- a row of logits held by the threads of a cluster of CTAs, shared by the
+// kernels of top_logits.cu, distill.cu and sample.cu.
+//
+// A row of V elements is cut into 16-byte vectors on 16-byte boundaries of the address space, so
+// a row that starts anywhere (an odd vocabulary) is read with wide loads all the same: only its
+// first and last vector can be partial, and their elements are read one by one.  A cluster of C
+// CTAs takes one row; CTA c takes a contiguous slice of the vectors, warp w of it a contiguous
+// part of that, so "in the order of the index" is the order (CTA, warp, vector row, lane, element).
+#pragma once
+#include <cooperative_groups.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cstdint>
+
+#include "common.cuh"
+#include "logits.cuh"
+
+namespace tbgb {
+namespace row {
+
+namespace cg = cooperative_groups;
+
+constexpr int NV = 8;  // 16-byte vectors a thread holds
+constexpr unsigned FULL = 0xffffffffu;
+
+__device__ __forceinline__ float neg_inff() { return __uint_as_float(0xff800000u); }
+
+// ---- element types -------------------------------------------------------------------------
+// KEY_BITS-bit ordered keys: k(a) < k(b) iff a < b, equal zeros, -inf lowest (NaN is replaced
+// by -inf before keys are taken).
+
+template <typename T>
+struct Elem;
+
+template <>
+struct Elem<float> {
+  static constexpr int EPV = 4, KEY_BITS = 32;
+  static constexpr uint32_t NEG_INF = 0xff800000u;
+  static __device__ __forceinline__ float get(const uint4& v, int e) {
+    return __uint_as_float(e == 0 ? v.x : e == 1 ? v.y : e == 2 ? v.z : v.w);
+  }
+  static __device__ __forceinline__ void set(uint4& v, int e, uint32_t bits) {
+    (e == 0 ? v.x : e == 1 ? v.y : e == 2 ? v.z : v.w) = bits;
+  }
+  static __device__ __forceinline__ uint32_t load_bits(const float* p) { return __float_as_uint(*p); }
+  static __device__ __forceinline__ float from_bits(uint32_t b) { return __uint_as_float(b); }
+  static __device__ __forceinline__ uint32_t to_bits(float f) { return __float_as_uint(f); }
+  static __device__ __forceinline__ uint32_t no_nan(uint32_t w) {
+    return __float_as_uint(fmaxf(__uint_as_float(w), neg_inff()));
+  }
+  static __device__ __forceinline__ uint32_t key(float z) {
+    const uint32_t u = __float_as_uint(z + 0.0f);
+    return u ^ (static_cast<uint32_t>(static_cast<int32_t>(u) >> 31) | 0x80000000u);
+  }
+  static __device__ __forceinline__ float unkey(uint32_t k) {
+    return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
+  }
+};
+
+template <typename T>
+struct Elem16 {
+  static constexpr int EPV = 8, KEY_BITS = 16;
+  static __device__ __forceinline__ uint32_t word(const uint4& v, int i) {
+    return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
+  }
+  static __device__ __forceinline__ void set(uint4& v, int e, uint32_t bits) {
+    uint32_t& w = (e >> 1) == 0 ? v.x : (e >> 1) == 1 ? v.y : (e >> 1) == 2 ? v.z : v.w;
+    w = (e & 1) ? (w & 0xffffu) | (bits << 16) : (w & 0xffff0000u) | bits;
+  }
+  static __device__ __forceinline__ uint32_t load_bits(const T* p) {
+    return *reinterpret_cast<const unsigned short*>(p);
+  }
+  static __device__ __forceinline__ uint32_t key_of_bits(uint32_t b) {
+    if (b == 0x8000u) b = 0;
+    return (b & 0x8000u) ? (~b & 0xffffu) : (b | 0x8000u);
+  }
+  static __device__ __forceinline__ uint32_t bits_of_key(uint32_t k) {
+    return (k & 0x8000u) ? (k & 0x7fffu) : (~k & 0xffffu);
+  }
+};
+
+template <>
+struct Elem<__nv_bfloat16> : Elem16<__nv_bfloat16> {
+  static constexpr uint32_t NEG_INF = 0xff80u;
+  static __device__ __forceinline__ float get(const uint4& v, int e) {
+    const uint32_t w = word(v, e >> 1);
+    return __uint_as_float((e & 1) ? (w & 0xffff0000u) : (w << 16));
+  }
+  static __device__ __forceinline__ float from_bits(uint32_t b) { return __uint_as_float(b << 16); }
+  static __device__ __forceinline__ uint32_t to_bits(float f) {
+    return __bfloat16_as_ushort(__float2bfloat16_rn(f));
+  }
+  static __device__ __forceinline__ uint32_t no_nan(uint32_t w) {
+    __nv_bfloat162 x = *reinterpret_cast<__nv_bfloat162*>(&w);
+    const uint32_t lo = 0xff80ff80u;
+    x = __hmax2(x, *reinterpret_cast<const __nv_bfloat162*>(&lo));
+    return *reinterpret_cast<uint32_t*>(&x);
+  }
+  static __device__ __forceinline__ uint32_t key(float z) { return key_of_bits(__float_as_uint(z) >> 16); }
+  static __device__ __forceinline__ float unkey(uint32_t k) { return from_bits(bits_of_key(k)); }
+};
+
+template <>
+struct Elem<__half> : Elem16<__half> {
+  static constexpr uint32_t NEG_INF = 0xfc00u;
+  static __device__ __forceinline__ float from_bits(uint32_t b) {
+    return __half2float(__ushort_as_half(static_cast<unsigned short>(b)));
+  }
+  static __device__ __forceinline__ float get(const uint4& v, int e) {
+    const uint32_t w = word(v, e >> 1);
+    return from_bits((e & 1) ? (w >> 16) : (w & 0xffffu));
+  }
+  static __device__ __forceinline__ uint32_t to_bits(float f) { return __half_as_ushort(__float2half_rn(f)); }
+  static __device__ __forceinline__ uint32_t no_nan(uint32_t w) {
+    __half2 x = *reinterpret_cast<__half2*>(&w);
+    const uint32_t lo = 0xfc00fc00u;
+    x = __hmax2(x, *reinterpret_cast<const __half2*>(&lo));
+    return *reinterpret_cast<uint32_t*>(&x);
+  }
+  static __device__ __forceinline__ uint32_t key(float z) { return key_of_bits(to_bits(z)); }
+  static __device__ __forceinline__ float unkey(uint32_t k) { return from_bits(bits_of_key(k)); }
+};
+
+// ---- a row's vectors -------------------------------------------------------------------------
+
+template <typename T>
+struct RowView {
+  const char* base;  // the row's first element, rounded down to 16 bytes
+  int off;           // elements between `base` and the row's first element
+  int vocab;
+  int nvec;  // vectors that hold at least one element of the row
+
+  __device__ __forceinline__ RowView(const T* p, int v) : vocab(v) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(p);
+    base = reinterpret_cast<const char*>(a & ~static_cast<uintptr_t>(15));
+    off = static_cast<int>((a & 15) / sizeof(T));
+    nvec = (off + v + Elem<T>::EPV - 1) / Elem<T>::EPV;
+  }
+  // index in the row of vector v's first element (negative in front of the row)
+  __device__ __forceinline__ int first(int v) const { return v * Elem<T>::EPV - off; }
+  __device__ __forceinline__ bool whole(int v) const {
+    const int j = first(v);
+    return j >= 0 && j + Elem<T>::EPV <= vocab;
+  }
+  // vector v; elements outside the row are -inf.  v < nvec.
+  __device__ __forceinline__ uint4 load(int v) const {
+    if (whole(v)) return __ldcs(reinterpret_cast<const uint4*>(base) + v);
+    uint4 r = none();
+    const T* e0 = reinterpret_cast<const T*>(base) + static_cast<long long>(v) * Elem<T>::EPV;
+    const int j0 = first(v);
+#pragma unroll
+    for (int e = 0; e < Elem<T>::EPV; ++e)
+      if (j0 + e >= 0 && j0 + e < vocab) Elem<T>::set(r, e, Elem<T>::load_bits(e0 + e));
+    return r;
+  }
+  static __device__ __forceinline__ uint4 none() {
+    constexpr uint32_t w = sizeof(T) == 4 ? Elem<T>::NEG_INF : Elem<T>::NEG_INF * 0x10001u;
+    return make_uint4(w, w, w, w);
+  }
+};
+
+// Elements whose mask bit is clear become -inf, NaN too.
+template <typename T>
+__device__ __forceinline__ void mask_vector(uint4& r, const RowView<T>& rv, int v, const uint64_t* mask) {
+  constexpr int EPV = Elem<T>::EPV;
+  r.x = Elem<T>::no_nan(r.x);
+  r.y = Elem<T>::no_nan(r.y);
+  r.z = Elem<T>::no_nan(r.z);
+  r.w = Elem<T>::no_nan(r.w);
+  if (!mask) return;
+  const int j0 = rv.first(v);
+  uint32_t bits = 0;
+  if (rv.whole(v)) {
+    const int sh = j0 & 63;
+    uint64_t w = mask[j0 >> 6] >> sh;
+    if (sh > 64 - EPV) w |= mask[(j0 >> 6) + 1] << (64 - sh);
+    bits = static_cast<uint32_t>(w);
+  } else {
+#pragma unroll
+    for (int e = 0; e < EPV; ++e) {
+      const int j = j0 + e;
+      if (j >= 0 && j < rv.vocab) bits |= static_cast<uint32_t>((mask[j >> 6] >> (j & 63)) & 1u) << e;
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < EPV; ++e)
+    if (!((bits >> e) & 1u)) Elem<T>::set(r, e, Elem<T>::NEG_INF);
+}
+
+// ---- a CTA's slice of a row -------------------------------------------------------------------
+// RES: the whole slice is in registers (at most NT * NV vectors), every pass reads it there.
+// Otherwise the slice is taken in tiles of NT * NV vectors that every pass loads again.
+
+template <typename T, int NT, bool RES>
+struct Slice {
+  static constexpr int EPV = Elem<T>::EPV;
+  static constexpr int TILE = NT * NV;
+  RowView<T> rv;
+  const uint64_t* mask;
+  int v0, v1;  // the slice's vectors
+  int tiles;
+  int per;     // vector rows a warp takes of a tile (<= NV)
+  uint4 r[NV];
+
+  __device__ __forceinline__ Slice(const T* p, int vocab, const uint64_t* m, int rank, int C) : rv(p, vocab), mask(m) {
+    const int each = (rv.nvec + C - 1) / C;
+    v0 = min(rank * each, rv.nvec);
+    v1 = min(v0 + each, rv.nvec);
+    const int n = v1 - v0;
+    tiles = RES ? 1 : (n + TILE - 1) / TILE;
+    per = min((n + NT - 1) / NT, NV);
+  }
+  __device__ __forceinline__ int vec(int tile, int i) const {
+    const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    return v0 + tile * TILE + (w * per + i) * 32 + lane;
+  }
+  __device__ __forceinline__ void load(int tile) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      r[i] = RowView<T>::none();
+      const int v = vec(tile, i);
+      if (i < per && v < v1) r[i] = rv.load(v);
+    }
+  }
+  __device__ __forceinline__ void clean(int tile) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int v = vec(tile, i);
+      if (i < per && v < v1) mask_vector<T>(r[i], rv, v, mask);
+    }
+  }
+  __device__ __forceinline__ void fetch(int tile) {
+    if (!RES) {
+      load(tile);
+      clean(tile);
+    }
+  }
+  // f(z, i, e) for every held element of a tile (also those outside the row: z = -inf)
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if (i < per) {
+#pragma unroll
+        for (int e = 0; e < EPV; ++e) f(Elem<T>::get(r[i], e), i, e);
+      }
+    }
+  }
+  __device__ __forceinline__ int index(int tile, int i, int e) const { return rv.first(vec(tile, i)) + e; }
+};
+
+// ---- reductions ---------------------------------------------------------------------------------
+
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(FULL, v, o));
+  return v;
+}
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(FULL, v, o);
+  return v;
+}
+__device__ __forceinline__ unsigned long long warp_sum(unsigned long long v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(FULL, v, o);
+  return v;
+}
+__device__ __forceinline__ int warp_sum(int v) { return static_cast<int>(__reduce_add_sync(FULL, static_cast<unsigned>(v))); }
+
+template <typename U>
+__device__ __forceinline__ U warp_inclusive(U v) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const U t = __shfl_up_sync(FULL, v, o);
+    if (lane >= o) v += t;
+  }
+  return v;
+}
+
+// ---- the softmax's running maximum and sum, in base 2 -------------------------------------------
+// Sums of 2^((z - m) * s) with m the largest z seen and s = log2(e) / T: z - m comes first, so a
+// row of the type's lowest values has exponents of 0 and no product overflows.
+
+struct MaxSum {
+  float m, s;
+  __device__ __forceinline__ void merge(float m2, float s2, float scale) {
+    if (m2 == neg_inff() || m == neg_inff()) {  // one side is empty: its sum is 0 (or NaN, which stays)
+      m = fmaxf(m, m2);
+      s += s2;
+      return;
+    }
+    const float top = fmaxf(m, m2);
+    s = s * (m == top ? 1.0f : exp2f((m - top) * scale)) + s2 * (m2 == top ? 1.0f : exp2f((m2 - top) * scale));
+    m = top;
+  }
+};
+
+// ---- launch ----------------------------------------------------------------------------------------
+
+// Cluster size for rows of `bytes` bytes on CTAs that hold `slice` bytes: the fewest CTAs that
+// hold the row, then more while the rows leave SMs without work and a thread keeps a vector.
+inline int cluster_size(long long bytes, long long slice, long long rows, int num_sms, int threads) {
+  int c = 1;
+  while (c < 8 && c * slice < bytes + 32) c *= 2;
+  while (c < 8 && rows * c * 2 <= num_sms && bytes / (c * 2) >= threads * 16) c *= 2;
+  return c;
+}
+
+template <typename K, typename A>
+cudaError_t launch_rows(K kernel, int threads, int cluster, size_t smem, const A& a, long long rows, cudaStream_t s) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(rows * cluster));
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = cluster;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, a);
+}
+
+}  // namespace row
+}  // namespace tbgb

@@ -1,0 +1,119 @@
+"""Rows of logits: a teacher's top logits, a student's distillation loss, sampled tokens.
+
+Functions over the library calls of the same names (tbgb_top_logits, tbgb_distill_*,
+tbgb_sample_tokens) for logits of any leading shape [..., vocab] on the device:
+
+* ``top_logits(logits, k)`` -> ``TopLogits``: what to keep of a teacher's logits;
+* ``distill_loss(logits, record)``: the loss of every position, differentiable by the logits;
+* ``sample_tokens(logits, u)``: one token per position from given uniform numbers.
+
+They enqueue on torch's current stream and do not wait; ``synchronize(device)`` waits and raises
+what the device reported (a token id outside the vocabulary, an id named twice in a record).
+"""
+from __future__ import annotations
+
+from dataclasses import dataclass
+
+from . import InvalidArgument, _torch
+
+
+def _ctx(device: int):
+    from .frame import _ctx as frame_ctx
+
+    return frame_ctx(device)
+
+
+def synchronize(device: int = 0):
+    """Wait for torch's current stream on `device` and raise what the kernels reported."""
+    _ctx(device).sync(_torch().cuda.current_stream(device))
+
+
+def _rows(t):
+    """[..., n] as [rows, n] without a copy."""
+    if t.dim() == 2:
+        return t
+    try:
+        return t.view(-1, t.shape[-1])
+    except RuntimeError:
+        raise InvalidArgument(7, "the leading dimensions must be viewable as one (make the tensor contiguous)") from None
+
+
+@dataclass
+class TopLogits:
+    """A teacher's record: per position the k largest logits (values) with their token ids, the
+    temperature it is meant for, and the log-sum-exp of all logits at that temperature (None: the
+    teacher is closed among its entries)."""
+
+    values: object
+    ids: object
+    lse: object
+    temperature: float
+
+    def closed(self) -> "TopLogits":
+        """The same entries as a distribution of their own."""
+        return TopLogits(self.values, self.ids, None, self.temperature)
+
+
+def top_logits(logits, k: int, temperature: float = 1.0, mask=None) -> TopLogits:
+    """The record of a teacher's logits [..., vocab]."""
+    lead = logits.shape[:-1]
+    out = _ctx(logits.device.index).top_logits(_rows(logits), k, temperature=temperature, mask=mask, sync=False)
+    return TopLogits(out["values"].view(*lead, k), out["ids"].view(*lead, k), out["lse"].view(lead), float(temperature))
+
+
+def _distill_function():
+    torch = _torch()
+
+    class DistillLoss(torch.autograd.Function):
+        @staticmethod
+        def forward(logits, values, ids, lse, temperature):
+            out = _ctx(logits.device.index).distill_loss(logits, ids, values, teacher_lse=lse, temperature=temperature,
+                                                         sync=False)
+            return out["loss"], out["stats"]
+
+        @staticmethod
+        def setup_context(ctx, inputs, output):
+            logits, values, ids, lse, ctx.temperature = inputs
+            ctx.mark_non_differentiable(output[1])
+            ctx.save_for_backward(logits, values, ids, lse, output[1])
+
+        @staticmethod
+        @torch.autograd.function.once_differentiable
+        def backward(ctx, grad_loss, _):
+            logits, values, ids, lse, stats = ctx.saved_tensors
+            grad = _ctx(logits.device.index).distill_grad(logits, ids, values, stats, grad_loss.float().contiguous(),
+                                                          teacher_lse=lse, temperature=ctx.temperature, sync=False)
+            return grad, None, None, None, None
+
+    return DistillLoss
+
+
+_function = None
+
+
+def distill_loss(logits, record: TopLogits):
+    """KL divergence of the student softmax(logits / T) from the recorded teacher at every position
+    (f32, the leading shape of `logits`), differentiable by the logits (once)."""
+    global _function
+    if _function is None:
+        _function = _distill_function()
+    lead = logits.shape[:-1]
+    lse = None if record.lse is None else record.lse.reshape(-1)
+    loss, _ = _function.apply(_rows(logits), _rows(record.values), _rows(record.ids), lse, record.temperature)
+    return loss.view(lead)
+
+
+def sample_tokens(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, mask=None):
+    """(tokens int32, log-probabilities f32) of the leading shape, from uniform numbers u of that shape.
+    The settings are numbers or tensors of that shape; see Context.sample_tokens."""
+    torch = _torch()
+    lead = logits.shape[:-1]
+
+    def flat(v, dtype):
+        return v.reshape(-1).to(dtype) if isinstance(v, torch.Tensor) else v
+
+    out = _ctx(logits.device.index).sample_tokens(
+        _rows(logits), flat(u, torch.float32), temperature=flat(temperature, torch.float32),
+        top_k=flat(top_k, torch.int32), top_p=flat(top_p, torch.float32), min_p=flat(min_p, torch.float32), mask=mask,
+        sync=False)
+    return out["tokens"].view(lead), out["logprobs"].view(lead)
