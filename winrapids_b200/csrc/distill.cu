@@ -12,6 +12,7 @@
 // A row whose student has no weight outside S, and one whose teacher has none there, have no such
 // outcome.  stats[r] = (log sum exp(z / T), the factor of q_j outside S) is what the backward pass
 // needs of the forward pass.
+#include <algorithm>
 #include <climits>
 
 #include "logits_row.cuh"
@@ -39,23 +40,487 @@ __device__ __forceinline__ void store_elem(void* grad, long long i, float g) {
     static_cast<unsigned short*>(grad)[i] = static_cast<unsigned short>(b);
 }
 
-// g[0 .. EPV) into the gradient's row at the places of vector v: 16 bytes at once where the
-// gradient's row starts at the same place between 16-byte boundaries as the logits' row.
+// The gradient's row.  Vectors go out 16 bytes at once where its first element lies at the same place
+// between 16-byte boundaries as that of the logits' row (the usual case: the same strides).
 template <typename T>
-__device__ __forceinline__ void store_vector(const RowView<T>& rv, char* grad_base, bool same, T* grad_row, int v,
-                                             const float* g) {
-  constexpr int EPV = Elem<T>::EPV;
-  if (same && rv.whole(v)) {
-    uint4 o = make_uint4(0, 0, 0, 0);
+struct GradRow {
+  T* row;
+  char* base;
+  bool same;
+
+  __device__ __forceinline__ GradRow(T* g, const T* z)
+      : row(g),
+        base(reinterpret_cast<char*>(reinterpret_cast<uintptr_t>(g) & ~static_cast<uintptr_t>(15))),
+        same(((reinterpret_cast<uintptr_t>(g) ^ reinterpret_cast<uintptr_t>(z)) & 15) == 0) {}
+  __device__ __forceinline__ void store(const RowView<T>& rv, int v, const uint4& g) const {
+    if (same && rv.whole(v)) {
+      __stcs(reinterpret_cast<uint4*>(base) + v, g);
+      return;
+    }
+    const int j0 = rv.first(v);
 #pragma unroll
-    for (int e = 0; e < EPV; ++e) Elem<T>::set(o, e, Elem<T>::to_bits(g[e]));
-    __stcs(reinterpret_cast<uint4*>(grad_base) + v, o);
+    for (int e = 0; e < Elem<T>::EPV; ++e)
+      if (j0 + e >= 0 && j0 + e < rv.vocab) store_elem<T>(row, j0 + e, Elem<T>::get(g, e));
+  }
+};
+
+// ---- loss and stats, and the gradient, in one pass over the logits -----------------------------------
+//
+// One cluster per row at a time, persistent over rows; CTA c holds its slice of a row in one of two
+// stages of shared memory.  Warp roles:
+//   producer   bulk-copies the slice of the next row as soon as its stage is free
+//   entries    loads the record of the next row, takes the slice's entries out of the stage (their logits are
+//              kept, their places become -inf, so the softmax's loop over the rest needs no test), and
+//              when the row is done writes the loss and the entries' gradients
+//   others     the running maximum and sum over the stage, the exchange of six numbers per CTA over
+//              distributed shared memory, then the gradient from the stage
+// The three overlap across rows and across the CTAs of an SM.
+
+__device__ __forceinline__ float scaled(float m, float s, float top, float scale) {
+  return m == neg_inff() || m == top ? s : s * power2((m - top) * scale);
+}
+
+struct RowPart {  // a CTA's part of a row
+  float m, s;     // largest logit outside S, sum of 2^((z - m) * scale)
+  float ms, ss;   // the same over S
+  float loss;     // sum p (log p - (z - ms) / T) over S
+  float p;        // sum p over S
+};
+
+struct RowSum {
+  float ref, total, s_in, s_out, loss, p;
+};
+
+// Every part's sums by the largest logit of all, the same in every lane: lane c takes CTA c's part
+// (a loop over them is a chain of latencies that stands between the two passes over a row).
+__device__ __forceinline__ RowSum row_sum(const RowPart* parts, int C, float scale) {
+  const int lane = threadIdx.x & 31;
+  RowPart p{neg_inff(), 0.0f, neg_inff(), 0.0f, 0.0f, 0.0f};
+  if ((lane & 7) < C) p = parts[lane & 7];
+  float m = fmaxf(p.m, p.ms);
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(FULL, m, o));
+  RowSum t;
+  t.ref = m == neg_inff() ? 0.0f : m;
+  t.s_out = scaled(p.m, p.s, m, scale);
+  t.s_in = scaled(p.ms, p.ss, m, scale);
+  t.p = p.p;
+  t.loss = p.loss;
+  if (p.p > 0.0f && p.ms > neg_inff()) t.loss -= p.p * ((p.ms - t.ref) * scale * kLn2);
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) {
+    t.s_out += __shfl_xor_sync(FULL, t.s_out, o);
+    t.s_in += __shfl_xor_sync(FULL, t.s_in, o);
+    t.p += __shfl_xor_sync(FULL, t.p, o);
+    t.loss += __shfl_xor_sync(FULL, t.loss, o);
+  }
+  t.total = t.s_in + t.s_out;
+  t.loss += t.p * log2f(t.total) * kLn2;
+  return t;
+}
+
+constexpr long long kWaitCycles = 4000000000ll;  // about 2 s
+
+// A bounded wait (KERR_TIMEOUT when it gives up) that also acquires what other CTAs of the cluster wrote.
+__device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, uint32_t* err) {
+  const uint32_t at = smem_u32(bar);
+  const long long t0 = clock64();  // (the global timer takes long to read)
+  for (uint32_t it = 1;; ++it) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(at), "r"(parity)
+        : "memory");
+    if (ok) return true;
+    if ((it & 255u) == 0 && clock64() - t0 > kWaitCycles) {
+      atomicOr(err, KERR_TIMEOUT);
+      return false;
+    }
+  }
+}
+
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// Six floats to `to` in CTA `cta` of the cluster, then an arrival on its barrier `bar`.
+__device__ __forceinline__ void send_part(RowPart* to, uint64_t* bar, int cta, const RowPart& p) {
+  uint32_t a, b;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(to)), "r"(cta));
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(b) : "r"(smem_u32(bar)), "r"(cta));
+  asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(a), "f"(p.m), "f"(p.s) : "memory");
+  asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(a + 8), "f"(p.ms), "f"(p.ss) : "memory");
+  asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(a + 16), "f"(p.loss), "f"(p.p) : "memory");
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(b) : "memory");
+}
+
+// A CTA's slice of a row: vectors v0 .. v0 + nv, those in [w0, w1) of the slice whole.
+template <typename T>
+struct RowSlice {
+  const T* z;
+  RowView<T> rv;
+  int v0, nv, w0, w1;
+
+  __device__ __forceinline__ RowSlice(const DistillArgs& a, long long r, int rank, int log2c)
+      : z(static_cast<const T*>(a.x.logits) + r * a.x.ld), rv(z, a.x.vocab) {
+    const int each = (rv.nvec + (1 << log2c) - 1) >> log2c;
+    v0 = min(rank * each, rv.nvec);
+    nv = min(each, rv.nvec - v0);
+    w0 = rv.off && v0 == 0 && nv > 0 ? 1 : 0;
+    w1 = nv > 0 && (rv.off + rv.vocab) % Elem<T>::EPV && v0 + nv == rv.nvec ? nv - 1 : nv;
+  }
+  __device__ __forceinline__ const char* at(int j) const { return rv.base + static_cast<long long>(v0 + j) * 16; }
+  __device__ __forceinline__ uint4 load(int j) const {
+    return j >= w0 && j < w1 ? __ldcs(reinterpret_cast<const uint4*>(at(j))) : rv.load_part(v0 + j);
+  }
+};
+
+#ifndef RING_NW
+#define RING_NW 4
+#endif
+constexpr int kRingWarps = RING_NW;                  // warps of the third role
+constexpr int kRingThreads = 32 * (kRingWarps + 2);  // and the producer's and the entries' warp
+
+// KR: entries of the record per lane of the entries' warp.
+template <typename T, int KR, bool GRAD>
+__global__ void __launch_bounds__(kRingThreads, KR > 4 ? 1 : 3) distill_kernel(const DistillArgs a, int cap) {
+  constexpr int EPV = Elem<T>::EPV, NW = kRingWarps, NT = 32 * NW;
+  extern __shared__ __align__(16) char ring[];  // two stages of `cap` bytes
+  // row n: index n & 1, phase (n >> 1) & 1
+  __shared__ __align__(8) uint64_t full[2], done[2], ready[2], counted[2], heard[2];
+  // four rows' parts: a peer may send row n + 1's while this CTA's entries' warp still reads row n - 1's
+  __shared__ __align__(8) RowPart parts[4][8];
+  __shared__ RowPart entries_part[2];
+  __shared__ float2 w_ms[NW];
+  cg::cluster_group cl = cg::this_cluster();
+  const int C = static_cast<int>(cl.num_blocks()), rank = static_cast<int>(cl.block_rank()), log2c = 31 - __clz(C);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const long long stride = gridDim.x >> log2c, rows = a.x.rows;
+  const float scale = kLog2e / a.temperature, inv_t = 1.0f / a.temperature;
+  const bool with_tail = a.teacher_lse != nullptr;
+  if (tid == 0) {
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&done[s], NW);
+      mbar_init(&ready[s], 1);
+      mbar_init(&counted[s], 1);
+      mbar_init(&heard[s], C);
+    }
+    mbar_fence_init();
+  }
+  cl.sync();
+
+  auto weight_of = [&](long long r) { return GRAD && r < rows ? a.weight[r] : 1.0f; };
+  int n = 0;  // rows taken so far (padding rows are not counted)
+  long long r = blockIdx.x >> log2c;
+  float w = weight_of(r);
+
+  if (warp == NW) {  // the producer
+    for (; r < rows; r += stride) {
+      const float next_w = weight_of(r + stride);
+      if (w != 0.0f) {
+        const int s = n & 1;
+        if (n >= 2 && !wait_phase(&done[s], ((n >> 1) - 1) & 1, a.err)) break;
+        const RowSlice<T> sl(a, r, rank, log2c);
+        char* stage = ring + s * cap;
+        // whole vectors by a bulk copy; the row's first and last vector, where partial, by elements
+        if (lane == 0) {
+          fence_proxy_async_smem();
+          if (sl.w1 > sl.w0) {
+            const uint32_t bytes = static_cast<uint32_t>(sl.w1 - sl.w0) * 16;
+            asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(&full[s])), "r"(bytes)
+                         : "memory");
+            bulk_g2s(stage + sl.w0 * 16, sl.at(sl.w0), bytes, &full[s]);
+          }
+        }
+        for (int side = 0; side < 2; ++side) {
+          const int j = side ? sl.nv - 1 : 0;
+          if ((side ? sl.w1 == sl.nv : sl.w0 == 0) || lane >= EPV) continue;
+          const int id = sl.rv.first(sl.v0 + j) + lane;
+          const uint32_t bits = id >= 0 && id < sl.rv.vocab ? Elem<T>::load_bits(sl.z + id) : Elem<T>::NEG_INF;
+          char* to = stage + j * 16 + lane * sizeof(T);
+          if (sizeof(T) == 4)
+            *reinterpret_cast<uint32_t*>(to) = bits;
+          else
+            *reinterpret_cast<unsigned short*>(to) = static_cast<unsigned short>(bits);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&full[s]);
+        ++n;
+      }
+      w = next_w;
+    }
+    // no copy may be in flight when the CTA ends
+    for (int k = max(n - 2, 0); k < n; ++k) wait_phase(&full[k & 1], (k >> 1) & 1, a.err);
     return;
   }
-  const int j0 = rv.first(v);
+
+  if (warp == NW + 1) {  // the entries
+    struct Entry {
+      int id;   // -1: none, or not in this CTA's slice
+      float z;  // the student's logit
+      float p;
+      float l;  // log2 p
+    };
+    Entry now[KR], before[KR];
+    int ahead_id[KR];
+    float ahead_t[KR], ahead_lse = 0.0f;
+    auto fetch = [&](long long row) {  // a row ahead of set(), so that nothing waits for it
+      if (row >= rows) return;
 #pragma unroll
-  for (int e = 0; e < EPV; ++e)
-    if (j0 + e >= 0 && j0 + e < rv.vocab) store_elem<T>(grad_row, j0 + e, g[e]);
+      for (int i = 0; i < KR; ++i)
+        if (lane + 32 * i < a.k) {
+          ahead_id[i] = a.ids[row * a.ids_ld + lane + 32 * i];
+          ahead_t[i] = teacher_logit(a, row * a.teacher_ld + lane + 32 * i);
+        }
+      if (with_tail) ahead_lse = a.teacher_lse[row];
+    };
+    auto set = [&](const RowSlice<T>& sl) {  // ids and p of the row that was fetched
+      const int lo = max(sl.rv.first(sl.v0), 0), hi = min(sl.rv.first(sl.v0 + sl.nv), a.x.vocab);
+      float t[KR], m = neg_inff(), sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < KR; ++i) {
+        int id = lane + 32 * i < a.k ? ahead_id[i] : -1;
+        if (id < -1 || id >= a.x.vocab) {
+          if (rank == 0) atomicOr(a.err, KERR_TOKEN_ID);
+          id = -1;
+        }
+        t[i] = id >= 0 ? ahead_t[i] : neg_inff();
+        now[i].id = id >= lo && id < hi ? id : -1;
+        m = fmaxf(m, t[i]);
+      }
+      if (with_tail) {
+#pragma unroll
+        for (int i = 0; i < KR; ++i) {
+          // t / T - lse: the quotient's own rounding is put back, it would be the error of log p
+          const float q = t[i] * inv_t;
+          const float rest = fabsf(q) < 1e30f ? fmaf(-q, a.temperature, t[i]) * inv_t : 0.0f;
+          now[i].l = t[i] == neg_inff() ? neg_inff() : (q - ahead_lse + rest) * kLog2e;
+        }
+      } else {
+        m = warp_max(m);
+        const float ref = m == neg_inff() ? 0.0f : m;
+#pragma unroll
+        for (int i = 0; i < KR; ++i) sum += power2((t[i] - ref) * scale);
+        const float l2 = log2f(warp_sum(sum));
+#pragma unroll
+        for (int i = 0; i < KR; ++i) now[i].l = m == neg_inff() ? neg_inff() : (t[i] - ref) * scale - l2;
+      }
+#pragma unroll
+      for (int i = 0; i < KR; ++i) now[i].p = power2(now[i].l);
+    };
+    long long last_r = -1;
+    int last_n = 0;
+    float last_w = 0.0f;
+    auto finish = [&]() {  // loss, stats and the entries' gradients of the row before
+      const int s = last_n & 1, phase = (last_n >> 1) & 1;
+      if (!wait_phase(&heard[s], phase, a.err)) return false;
+      const RowSum t = row_sum(parts[last_n & 3], C, scale);
+      const float inv = __fdividef(1.0f, t.total);
+      if (rank == 0 && lane == 0) {
+        float loss = t.loss, off = 1.0f;
+        if (with_tail && t.p < 1.0f && t.s_out > 0.0f) {
+          const float q_in = t.s_in * inv, q_out = t.s_out * inv;
+          const float lq = q_in < 0.5f ? log1pf(-q_in) : logf(q_out);
+          loss += (1.0f - t.p) * (log1pf(-t.p) - lq);
+          off = __fdividef(t.p - q_in, q_out);
+        }
+        a.loss[last_r] = loss;
+        a.stats[2 * last_r] = t.total > 0.0f ? t.ref / a.temperature + logf(t.total) : neg_inff() + t.total;
+        a.stats[2 * last_r + 1] = off;
+      }
+      if (!GRAD) return true;
+      if (!wait_phase(&done[s], phase, a.err)) return false;  // over what the others have stored
+      T* g = static_cast<T*>(a.grad) + last_r * a.grad_ld;
+      const float wt = last_w * inv_t;
+#pragma unroll
+      for (int i = 0; i < KR; ++i)
+        if (before[i].id >= 0)
+          store_elem<T>(g, before[i].id, wt * (power2((before[i].z - t.ref) * scale) * inv - before[i].p));
+      return true;
+    };
+    fetch(r);
+    if (r < rows && w != 0.0f) set(RowSlice<T>(a, r, rank, log2c));
+    fetch(r + stride);
+    for (; r < rows; r += stride) {
+      const float next_w = weight_of(r + stride);
+      if (w != 0.0f) {
+        const int s = n & 1, phase = (n >> 1) & 1;
+        const RowSlice<T> sl(a, r, rank, log2c);
+        const int f0 = sl.rv.first(sl.v0);
+        if (!wait_phase(&full[s], phase, a.err)) break;
+        T* stage = reinterpret_cast<T*>(ring + s * cap);
+        auto put = [&](int j, uint32_t bits) {
+          if (sizeof(T) == 4)
+            reinterpret_cast<volatile uint32_t*>(stage)[j] = bits;
+          else
+            reinterpret_cast<volatile unsigned short*>(stage)[j] = static_cast<unsigned short>(bits);
+        };
+        // z out of the stage; k into its place, to see whether another entry has the same place; then -inf
+#pragma unroll
+        for (int i = 0; i < KR; ++i)
+          if (now[i].id >= 0) now[i].z = Elem<T>::from_bits(Elem<T>::load_bits(stage + (now[i].id - f0)));
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < KR; ++i)
+          if (now[i].id >= 0) put(now[i].id - f0, lane + 32 * i);
+        __syncwarp();
+        bool twice = false;
+#pragma unroll
+        for (int i = 0; i < KR; ++i)
+          if (now[i].id >= 0) twice |= Elem<T>::load_bits(stage + (now[i].id - f0)) != static_cast<uint32_t>(lane + 32 * i);
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < KR; ++i)
+          if (now[i].id >= 0) put(now[i].id - f0, Elem<T>::NEG_INF);
+        fence_proxy_async_smem();  // before the stage's next bulk copy
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ready[s]);
+        if (twice) atomicOr(a.err, KERR_TOKEN_TWICE);
+        float ms = neg_inff(), ss = 0.0f, loss = 0.0f, ps = 0.0f;
+#pragma unroll
+        for (int i = 0; i < KR; ++i)
+          if (now[i].id >= 0) ms = fmaxf(ms, now[i].z);
+        ms = warp_max(ms);
+        const float ref = ms == neg_inff() ? 0.0f : ms;
+#pragma unroll
+        for (int i = 0; i < KR; ++i)
+          if (now[i].id >= 0) {
+            const float d = (now[i].z - ref) * scale;
+            ss += power2(d);
+            if (now[i].p != 0.0f) loss += now[i].p * ((now[i].l - d) * kLn2);
+            ps += now[i].p;
+          }
+        ss = warp_sum(ss);
+        loss = warp_sum(loss);
+        ps = warp_sum(ps);
+        if (lane == 0) {
+          entries_part[s] = RowPart{neg_inff(), 0.0f, ms, ss, loss, ps};
+          mbar_arrive(&counted[s]);
+        }
+        if (last_r >= 0 && !finish()) break;
+#pragma unroll
+        for (int i = 0; i < KR; ++i) before[i] = now[i];
+        last_r = r;
+        last_n = n;
+        last_w = w;
+        ++n;
+      } else if (rank == 0 && lane == 0) {
+        a.loss[r] = 0.0f;
+        a.stats[2 * r] = 0.0f;
+        a.stats[2 * r + 1] = 1.0f;
+      }
+      if (r + stride < rows && next_w != 0.0f) set(RowSlice<T>(a, r + stride, rank, log2c));
+      fetch(r + 2 * stride);
+      w = next_w;
+    }
+    if (last_r >= 0 && r >= rows) finish();
+    return;
+  }
+
+  // the softmax and the gradient
+  const float2 scale2 = make_float2(scale, scale);
+  for (; r < rows; r += stride) {
+    const float next_w = weight_of(r + stride);
+    const RowSlice<T> sl(a, r, rank, log2c);
+    const GradRow<T> out(GRAD ? static_cast<T*>(a.grad) + r * a.grad_ld : nullptr, sl.z);
+    if (w == 0.0f) {
+      for (int j = tid; j < sl.nv; j += NT) out.store(sl.rv, sl.v0 + j, make_uint4(0, 0, 0, 0));
+      w = next_w;
+      continue;
+    }
+    const int s = n & 1, phase = (n >> 1) & 1, nv = sl.nv;
+    const uint4* stage = reinterpret_cast<const uint4*>(ring + s * cap);
+    if (!wait_phase(&full[s], phase, a.err) || !wait_phase(&ready[s], phase, a.err)) return;
+
+    // four vectors at a time; the sum is scaled when they raise the maximum
+    float m = neg_inff();
+    float2 sum = make_float2(0.0f, 0.0f);
+    auto take = [&](const uint4 (&x)[4]) {
+      float top = m;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) top = fmaxf(top, Elem<T>::vmax(x[i]));
+      if (top > m) {
+        const float f = m == neg_inff() ? 1.0f : power2((m - top) * scale);
+        sum = mul2(sum, make_float2(f, f));
+        m = top;
+      }
+      const float ref = m == neg_inff() ? 0.0f : m;
+      const float2 minus_ref = make_float2(-ref, -ref);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < Elem<T>::PAIRS; ++j) sum = add2(sum, power2(Elem<T>::pair(x[i], j), minus_ref, scale2));
+    };
+    int v = tid;
+    for (; v + 3 * NT < nv; v += 4 * NT) {
+      const uint4 x[4] = {stage[v], stage[v + NT], stage[v + 2 * NT], stage[v + 3 * NT]};
+      take(x);
+    }
+    if (v < nv) {
+      uint4 x[4] = {stage[v], RowView<T>::none(), RowView<T>::none(), RowView<T>::none()};
+#pragma unroll
+      for (int i = 1; i < 4; ++i)
+        if (v + i * NT < nv) x[i] = stage[v + i * NT];
+      take(x);
+    }
+    __syncwarp();
+    if (!GRAD && lane == 0) mbar_arrive(&done[s]);
+    const float m_w = warp_max(m);
+    const float s_w = warp_sum(scaled(m, sum.x + sum.y, m_w, scale));
+    if (lane == 0) w_ms[warp] = make_float2(m_w, s_w);
+    asm volatile("bar.sync 1, %0;" ::"n"(NT) : "memory");
+    if (warp == 0) {
+      const float2 ms = lane < NW ? w_ms[lane] : make_float2(neg_inff(), 0.0f);
+      if (!wait_phase(&counted[s], phase, a.err)) return;
+      RowPart part = entries_part[s];
+      part.m = ms.x;
+#pragma unroll
+      for (int o = NW > 8 ? 8 : 4; o > 0; o >>= 1) part.m = fmaxf(part.m, __shfl_xor_sync(FULL, part.m, o));
+      part.s = scaled(ms.x, ms.y, part.m, scale);
+#pragma unroll
+      for (int o = NW > 8 ? 8 : 4; o > 0; o >>= 1) part.s += __shfl_xor_sync(FULL, part.s, o);
+      if (lane < C) send_part(&parts[n & 3][rank], &heard[s], lane, part);
+    }
+    if (!wait_phase(&heard[s], phase, a.err)) return;
+    if (GRAD) {
+      const RowSum t = row_sum(parts[n & 3], C, scale);
+      const float inv = __fdividef(1.0f, t.total);
+      float f = w * inv_t * inv;
+      if (with_tail && t.p < 1.0f && t.s_out > 0.0f)
+        f = w * inv_t * __fdividef(t.p - t.s_in * inv, t.s_out);  // (p(S) - q(S)) / q_r / total
+      const float2 minus_ref = make_float2(-t.ref, -t.ref), f2 = make_float2(f, f);
+      auto give = [&](const uint4& x) {
+        uint4 g;
+#pragma unroll
+        for (int j = 0; j < Elem<T>::PAIRS; ++j)
+          Elem<T>::set_pair(g, j, mul2(power2(Elem<T>::pair(x, j), minus_ref, scale2), f2));
+        return g;
+      };
+      if (out.same) {
+        // whole vectors at once, the row's partial ends by elements
+        uint4* to = reinterpret_cast<uint4*>(out.base) + sl.v0;
+        int v = tid + sl.w0;
+        for (; v + 3 * NT < sl.w1; v += 4 * NT) {
+          const uint4 x[4] = {stage[v], stage[v + NT], stage[v + 2 * NT], stage[v + 3 * NT]};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) __stcs(to + v + i * NT, give(x[i]));
+        }
+        for (; v < sl.w1; v += NT) __stcs(to + v, give(stage[v]));
+        if (tid == 0 && sl.w0 > 0) out.store(sl.rv, sl.v0, give(stage[0]));
+        if (tid == NT - 1 && sl.w1 < nv && sl.w1 >= sl.w0) out.store(sl.rv, sl.v0 + nv - 1, give(stage[nv - 1]));
+      } else {
+        for (int v = tid; v < nv; v += NT) out.store(sl.rv, sl.v0 + v, give(stage[v]));
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&done[s]);
+    }
+    ++n;
+    w = next_w;
+  }
 }
 
 // The row's entries in shared memory: id (-1: none, also an id outside the vocabulary, which is
@@ -104,9 +569,10 @@ struct Part {  // a CTA's part of the student's softmax
   float in;    // sum over S
 };
 
-// loss and stats, and with GRAD the gradient; one cluster per row.  GRAD needs RES.
-template <typename T, int NT, bool RES, bool GRAD>
-__global__ void __launch_bounds__(NT) distill_kernel(const DistillArgs a) {
+// Loss and stats of rows too long for the stages above: a cluster per row, the slices read in tiles, a bit
+// per element of the slice for the entries.
+template <typename T, int NT>
+__global__ void __launch_bounds__(NT) distill_wide_kernel(const DistillArgs a) {
   constexpr int NW = NT / 32, EPV = Elem<T>::EPV;
   extern __shared__ uint32_t smem[];
   __shared__ float w_m[NW], w_s[NW];
@@ -117,18 +583,9 @@ __global__ void __launch_bounds__(NT) distill_kernel(const DistillArgs a) {
   const long long r = blockIdx.x / C;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const T* z_row = static_cast<const T*>(a.x.logits) + r * a.x.ld;
-  T* g_row = GRAD ? static_cast<T*>(a.grad) + r * a.grad_ld : nullptr;
-  Slice<T, NT, RES> sl(z_row, a.x.vocab, nullptr, rank, C);
-  const bool same = GRAD && ((reinterpret_cast<uintptr_t>(g_row) ^ reinterpret_cast<uintptr_t>(z_row)) & 15) == 0;
-  char* g_base = reinterpret_cast<char*>(reinterpret_cast<uintptr_t>(g_row) & ~static_cast<uintptr_t>(15));
+  Slice<T, NT, false> sl(z_row, a.x.vocab, nullptr, rank, C);
   const float w = a.weight ? a.weight[r] : 1.0f;
   if (w == 0.0f) {  // a padding row: not read
-    if (GRAD) {
-      float zero[EPV];
-#pragma unroll
-      for (int e = 0; e < EPV; ++e) zero[e] = 0.0f;
-      for (int v = sl.v0 + tid; v < sl.v1; v += NT) store_vector<T>(sl.rv, g_base, same, g_row, v, zero);
-    }
     if (rank == 0 && tid == 0) {
       a.loss[r] = 0.0f;
       a.stats[2 * r] = 0.0f;
@@ -136,7 +593,6 @@ __global__ void __launch_bounds__(NT) distill_kernel(const DistillArgs a) {
     }
     return;
   }
-  if (RES) sl.load(0);
 
   // the entries; bit (vector - v0) * EPV + e marks an element of S in this CTA's slice
   Entries en;
@@ -172,7 +628,7 @@ __global__ void __launch_bounds__(NT) distill_kernel(const DistillArgs a) {
   const float scale = kLog2e / a.temperature;
   float m_w = neg_inff(), s_w = 0.0f;
   for (int t = 0; t < sl.tiles; ++t) {
-    if (!RES) sl.load(t);
+    sl.load(t);
     float m = neg_inff(), s = 0.0f;
     sl.each([&](float z, int, int) { m = fmaxf(m, z); });
     m = warp_max(m);
@@ -252,30 +708,11 @@ __global__ void __launch_bounds__(NT) distill_kernel(const DistillArgs a) {
       a.stats[2 * r + 1] = off;
     }
   }
-  if (!GRAD) return;
-
-  const float wt = w / a.temperature, f = wt / total;
-  const float f_off = f * off;
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int v = sl.vec(0, i);
-    if (i < sl.per && v < sl.v1) {
-      float g[EPV];
-#pragma unroll
-      for (int e = 0; e < EPV; ++e) g[e] = exp2f((Elem<T>::get(sl.r[i], e) - ref) * scale) * f_off;
-      store_vector<T>(sl.rv, g_base, same, g_row, v, g);
-    }
-  }
-  __syncthreads();  // the entries' gradients go over what was just stored
-  for (int k = tid; k < a.k; k += NT)
-    if (en.id[k] >= lo && en.id[k] < hi)
-      store_elem<T>(g_row, en.id[k], exp2f((en.z[k] - ref) * scale) * f - wt * en.p[k]);
 }
 
 // The gradient from a forward pass's stats: one CTA per tile of NT * NV vectors of a row.
 template <typename T, int NT>
-__global__ void __launch_bounds__(NT) distill_grad_kernel(const DistillArgs a, int tiles) {
-  constexpr int EPV = Elem<T>::EPV;
+__global__ void __launch_bounds__(NT, 1024 / NT) distill_grad_kernel(const DistillArgs a, int tiles) {
   extern __shared__ uint32_t smem[];
   const long long r = blockIdx.x / tiles;
   const int rank = static_cast<int>(blockIdx.x - r * tiles);
@@ -283,14 +720,10 @@ __global__ void __launch_bounds__(NT) distill_grad_kernel(const DistillArgs a, i
   const T* z_row = static_cast<const T*>(a.x.logits) + r * a.x.ld;
   T* g_row = static_cast<T*>(a.grad) + r * a.grad_ld;
   Slice<T, NT, true> sl(z_row, a.x.vocab, nullptr, rank, tiles);
-  const bool same = ((reinterpret_cast<uintptr_t>(g_row) ^ reinterpret_cast<uintptr_t>(z_row)) & 15) == 0;
-  char* g_base = reinterpret_cast<char*>(reinterpret_cast<uintptr_t>(g_row) & ~static_cast<uintptr_t>(15));
+  const GradRow<T> out(g_row, z_row);
   const float w = a.weight[r];
   if (w == 0.0f) {
-    float zero[EPV];
-#pragma unroll
-    for (int e = 0; e < EPV; ++e) zero[e] = 0.0f;
-    for (int v = sl.v0 + tid; v < sl.v1; v += NT) store_vector<T>(sl.rv, g_base, same, g_row, v, zero);
+    for (int v = sl.v0 + tid; v < sl.v1; v += NT) out.store(sl.rv, v, make_uint4(0, 0, 0, 0));
     return;
   }
   sl.load(0);
@@ -312,16 +745,21 @@ __global__ void __launch_bounds__(NT) distill_grad_kernel(const DistillArgs a, i
   __syncthreads();
   if (tid < 32) entry_probs(a, en, r);
   const float inv_t = 1.0f / a.temperature, lse = a.stats[2 * r], off = a.stats[2 * r + 1];
-  const float wt = w * inv_t, f_off = wt * off;
-  auto q = [&](float z) { return exp2f((z * inv_t - lse) * kLog2e); };
+  const float wt = w * inv_t;
+  auto q = [&](float z) { return power2((z * inv_t - lse) * kLog2e); };
+  const float2 inv2 = make_float2(inv_t, inv_t), minus_lse = make_float2(-lse, -lse),
+               log2e2 = make_float2(kLog2e, kLog2e), f_off = make_float2(wt * off, wt * off);
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int v = sl.vec(0, i);
     if (i < sl.per && v < sl.v1) {
-      float g[EPV];
+      uint4 g;
 #pragma unroll
-      for (int e = 0; e < EPV; ++e) g[e] = q(Elem<T>::get(sl.r[i], e)) * f_off;
-      store_vector<T>(sl.rv, g_base, same, g_row, v, g);
+      for (int j = 0; j < Elem<T>::PAIRS; ++j) {
+        const float2 d = mul2(add2(mul2(Elem<T>::pair(sl.r[i], j), inv2), minus_lse), log2e2);
+        Elem<T>::set_pair(g, j, mul2(make_float2(power2(d.x), power2(d.y)), f_off));
+      }
+      out.store(sl.rv, v, g);
     }
   }
   __syncthreads();
@@ -339,30 +777,42 @@ cudaError_t allow_smem(K kernel, size_t bytes) {
 template <typename T>
 cudaError_t launch(const DistillArgs& a, bool with_loss, bool with_grad, int num_sms, cudaStream_t s,
                    uint64_t* launches) {
-  constexpr int NT = 512;
-  constexpr long long SLICE = NT * NV * 16;
   const long long bytes = static_cast<long long>(a.x.vocab) * sizeof(T);
-  const size_t entries = static_cast<size_t>(a.k) * 12;
-  cudaError_t e = cudaSuccess;
   if (with_loss) {
-    const int c = cluster_size(bytes, SLICE, a.x.rows, num_sms, NT);
-    const bool res = c * SLICE >= bytes + 32;
-    const long long nvec = bytes / 16 + 2;
-    const size_t smem = entries + ((nvec + c - 1) / c * Elem<T>::EPV + 31) / 32 * 4;
-    auto kernel = res ? (with_grad ? distill_kernel<T, NT, true, true> : distill_kernel<T, NT, true, false>)
-                      : distill_kernel<T, NT, false, false>;
-    e = allow_smem(kernel, smem);
-    if (e == cudaSuccess) e = launch_rows(kernel, NT, c, smem, a, a.x.rows, s);
+    // the fewest CTAs whose two stages leave room for three CTAs on an SM, more while rows are few
+    const bool aligned = reinterpret_cast<uintptr_t>(a.x.logits) % 16 == 0 && a.x.ld * sizeof(T) % 16 == 0;
+    const long long nvec = aligned ? (bytes + 15) / 16 : bytes / 16 + 2;
+    int c = 1;
+    while (c < 8 && 2 * ((nvec + c - 1) / c * 16) > 72 * 1024) c *= 2;
+    while (c < 8 && a.x.rows * c * 2 <= 2 * num_sms && nvec / (c * 2) >= 128) c *= 2;
+    const long long cap = (nvec + c - 1) / c * 16;
+    if (2 * cap <= 222 * 1024) {
+      const size_t smem = static_cast<size_t>(2 * cap);
+      auto kernel = a.k <= 128 ? (with_grad ? distill_kernel<T, 4, true> : distill_kernel<T, 4, false>)
+                               : (with_grad ? distill_kernel<T, 32, true> : distill_kernel<T, 32, false>);
+      int held = 0;
+      cudaError_t e = allow_smem(kernel, smem);
+      if (e == cudaSuccess) e = resident_clusters(kernel, kRingThreads, c, smem, &held);
+      if (e == cudaSuccess)
+        e = launch_rows(kernel, kRingThreads, c, smem, std::min(a.x.rows, static_cast<long long>(std::max(held, 1))), s,
+                        a, static_cast<int>(cap));
+      if (e == cudaSuccess) (*launches)++;
+      return e;
+    }
+    constexpr int NT = 512;
+    const size_t wide = static_cast<size_t>(a.k) * 12 + ((nvec + c - 1) / c * Elem<T>::EPV + 31) / 32 * 4;
+    cudaError_t e = allow_smem(distill_wide_kernel<T, NT>, wide);
+    if (e == cudaSuccess) e = launch_rows(distill_wide_kernel<T, NT>, NT, c, wide, a.x.rows, s, a);
     if (e != cudaSuccess) return e;
     (*launches)++;
-    if (res || !with_grad) return e;
   }
-  if (with_grad) {
-    const int tiles = static_cast<int>((bytes + 32 + SLICE - 1) / SLICE);
-    distill_grad_kernel<T, NT><<<static_cast<unsigned>(a.x.rows * tiles), NT, entries, s>>>(a, tiles);
-    e = cudaGetLastError();
-    if (e == cudaSuccess) (*launches)++;
-  }
+  if (!with_grad) return cudaSuccess;
+  constexpr int NT = 512;
+  constexpr long long TILE = NT * NV * 16;
+  const int tiles = static_cast<int>((bytes + 32 + TILE - 1) / TILE);
+  distill_grad_kernel<T, NT><<<static_cast<unsigned>(a.x.rows * tiles), NT, static_cast<size_t>(a.k) * 12, s>>>(a, tiles);
+  const cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess) (*launches)++;
   return e;
 }
 

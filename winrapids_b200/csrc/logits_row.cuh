@@ -43,6 +43,18 @@ struct Elem<float> {
   static __device__ __forceinline__ void set(uint4& v, int e, uint32_t bits) {
     (e == 0 ? v.x : e == 1 ? v.y : e == 2 ? v.z : v.w) = bits;
   }
+  static constexpr int PAIRS = 2;
+  static __device__ __forceinline__ float2 pair(const uint4& v, int i) {
+    return i == 0 ? make_float2(__uint_as_float(v.x), __uint_as_float(v.y))
+                  : make_float2(__uint_as_float(v.z), __uint_as_float(v.w));
+  }
+  static __device__ __forceinline__ void set_pair(uint4& v, int i, float2 f) {
+    (i == 0 ? v.x : v.z) = __float_as_uint(f.x);
+    (i == 0 ? v.y : v.w) = __float_as_uint(f.y);
+  }
+  static __device__ __forceinline__ float vmax(const uint4& v) {
+    return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
+  }
   static __device__ __forceinline__ uint32_t load_bits(const float* p) { return __float_as_uint(*p); }
   static __device__ __forceinline__ float from_bits(uint32_t b) { return __uint_as_float(b); }
   static __device__ __forceinline__ uint32_t to_bits(float f) { return __float_as_uint(f); }
@@ -60,7 +72,7 @@ struct Elem<float> {
 
 template <typename T>
 struct Elem16 {
-  static constexpr int EPV = 8, KEY_BITS = 16;
+  static constexpr int EPV = 8, KEY_BITS = 16, PAIRS = 4;
   static __device__ __forceinline__ uint32_t word(const uint4& v, int i) {
     return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
   }
@@ -87,6 +99,22 @@ struct Elem<__nv_bfloat16> : Elem16<__nv_bfloat16> {
     const uint32_t w = word(v, e >> 1);
     return __uint_as_float((e & 1) ? (w & 0xffff0000u) : (w << 16));
   }
+  static __device__ __forceinline__ float2 pair(const uint4& v, int i) {
+    const uint32_t w = word(v, i);
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  }
+  static __device__ __forceinline__ void set_pair(uint4& v, int i, float2 f) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(f.x, f.y);
+    (i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w) = *reinterpret_cast<const uint32_t*>(&h);
+  }
+  static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    const __nv_bfloat162 h = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  static __device__ __forceinline__ float vmax(const uint4& v) {
+    const uint32_t m = max2(max2(v.x, v.y), max2(v.z, v.w));
+    return fmaxf(__uint_as_float(m << 16), __uint_as_float(m & 0xffff0000u));
+  }
   static __device__ __forceinline__ float from_bits(uint32_t b) { return __uint_as_float(b << 16); }
   static __device__ __forceinline__ uint32_t to_bits(float f) {
     return __bfloat16_as_ushort(__float2bfloat16_rn(f));
@@ -107,6 +135,23 @@ struct Elem<__half> : Elem16<__half> {
   static __device__ __forceinline__ float from_bits(uint32_t b) {
     return __half2float(__ushort_as_half(static_cast<unsigned short>(b)));
   }
+  static __device__ __forceinline__ float2 pair(const uint4& v, int i) {
+    const uint32_t w = word(v, i);
+    return __half22float2(*reinterpret_cast<const __half2*>(&w));
+  }
+  static __device__ __forceinline__ void set_pair(uint4& v, int i, float2 f) {
+    const __half2 h = __floats2half2_rn(f.x, f.y);
+    (i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w) = *reinterpret_cast<const uint32_t*>(&h);
+  }
+  static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    const __half2 h = __hmax2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  static __device__ __forceinline__ float vmax(const uint4& v) {
+    const uint32_t m = max2(max2(v.x, v.y), max2(v.z, v.w));
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&m));
+    return fmaxf(f.x, f.y);
+  }
   static __device__ __forceinline__ float get(const uint4& v, int e) {
     const uint32_t w = word(v, e >> 1);
     return from_bits((e & 1) ? (w >> 16) : (w & 0xffffu));
@@ -121,6 +166,42 @@ struct Elem<__half> : Elem16<__half> {
   static __device__ __forceinline__ uint32_t key(float z) { return key_of_bits(to_bits(z)); }
   static __device__ __forceinline__ float unkey(uint32_t k) { return from_bits(bits_of_key(k)); }
 };
+
+// ---- two 32-bit numbers at a time ------------------------------------------------------------
+// Blackwell's packed f32 instructions do the softmax's subtraction, scaling and additions on two
+// elements per issue slot, rounding each as the single instructions do.
+
+__device__ __forceinline__ uint64_t pack2(float2 a) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a.x), "f"(a.y));
+  return r;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a));
+  return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pack2(a)), "l"(pack2(b)));
+  return unpack2(r);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pack2(a)), "l"(pack2(b)));
+  return unpack2(r);
+}
+// 2^x; results below 2^-126 are 0
+__device__ __forceinline__ float power2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+// 2^((z - ref) * scale)
+__device__ __forceinline__ float2 power2(float2 z, float2 minus_ref, float2 scale) {
+  const float2 d = mul2(add2(z, minus_ref), scale);
+  return make_float2(power2(d.x), power2(d.y));
+}
 
 // ---- a row's vectors -------------------------------------------------------------------------
 
@@ -144,8 +225,8 @@ struct RowView {
     return j >= 0 && j + Elem<T>::EPV <= vocab;
   }
   // vector v; elements outside the row are -inf.  v < nvec.
-  __device__ __forceinline__ uint4 load(int v) const {
-    if (whole(v)) return __ldcs(reinterpret_cast<const uint4*>(base) + v);
+  __device__ __forceinline__ uint4 load_whole(int v) const { return __ldcs(reinterpret_cast<const uint4*>(base) + v); }
+  __device__ __forceinline__ uint4 load_part(int v) const {
     uint4 r = none();
     const T* e0 = reinterpret_cast<const T*>(base) + static_cast<long long>(v) * Elem<T>::EPV;
     const int j0 = first(v);
@@ -216,11 +297,21 @@ struct Slice {
     return v0 + tile * TILE + (w * per + i) * 32 + lane;
   }
   __device__ __forceinline__ void load(int tile) {
+    // whole vectors lie between the row's first and last; each of those two is one thread's
+    const int head = rv.off ? 1 : 0, tail = (rv.off + rv.vocab) % EPV ? rv.nvec - 1 : rv.nvec;
+    const int end = min(v1, tail);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       r[i] = RowView<T>::none();
       const int v = vec(tile, i);
-      if (i < per && v < v1) r[i] = rv.load(v);
+      if (i < per && v < end && v >= head) r[i] = rv.load_whole(v);
+    }
+    if (head && v0 == 0 && tile == 0 && threadIdx.x == 0 && v1 > 0) r[0] = rv.load_part(0);
+    if (tail < v1) {  // (after a head that is the whole row: the same vector again)
+      const uint4 last = vec(tile, 0) <= tail && vec(tile, per - 1) >= tail ? rv.load_part(tail) : RowView<T>::none();
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (i < per && vec(tile, i) == tail) r[i] = last;
     }
   }
   __device__ __forceinline__ void clean(int tile) {
@@ -309,21 +400,38 @@ inline int cluster_size(long long bytes, long long slice, long long rows, int nu
   return c;
 }
 
-template <typename K, typename A>
-cudaError_t launch_rows(K kernel, int threads, int cluster, size_t smem, const A& a, long long rows, cudaStream_t s) {
+struct ClusterLaunch {
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(rows * cluster));
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
   cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = cluster;
-  at[0].val.clusterDim.y = 1;
-  at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, a);
+  ClusterLaunch(int threads, int cluster, size_t smem, long long clusters, cudaStream_t s) {
+    cfg.gridDim = dim3(static_cast<unsigned>(clusters * cluster));
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = cluster;
+    at[0].val.clusterDim.y = 1;
+    at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+  }
+};
+
+// `clusters` clusters of `cluster` CTAs.
+template <typename... P, typename... A>
+cudaError_t launch_rows(void (*kernel)(P...), int threads, int cluster, size_t smem, long long clusters, cudaStream_t s,
+                        const A&... args) {
+  ClusterLaunch l(threads, cluster, smem, clusters, s);
+  return cudaLaunchKernelEx(&l.cfg, kernel, args...);
+}
+
+// Clusters of a persistent kernel that the device holds at once.  A cluster lies within one GPC, so
+// this is less than the SMs' room divided by its size (C = 8: 48 instead of 55), and one cluster
+// more than it would run after the others: twice the time.
+template <typename... P>
+cudaError_t resident_clusters(void (*kernel)(P...), int threads, int cluster, size_t smem, int* n) {
+  ClusterLaunch l(threads, cluster, smem, 1, nullptr);
+  return cudaOccupancyMaxActiveClusters(n, kernel, &l.cfg);
 }
 
 }  // namespace row

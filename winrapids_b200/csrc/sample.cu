@@ -275,8 +275,8 @@ cudaError_t launch(const SampleArgs& a, int num_sms, cudaStream_t s) {
   constexpr int NT = 512;
   const int c = cluster_size(bytes, NT * NV * 16, a.x.rows, num_sms, NT);
   const bool res = static_cast<long long>(c) * NT * NV * 16 >= bytes + 32;
-  if (res) return launch_rows(sample_kernel<T, NT, true>, NT, c, 0, a, a.x.rows, s);
-  return launch_rows(sample_kernel<T, NT, false>, NT, c, 0, a, a.x.rows, s);
+  if (res) return launch_rows(sample_kernel<T, NT, true>, NT, c, 0, a.x.rows, s, a);
+  return launch_rows(sample_kernel<T, NT, false>, NT, c, 0, a.x.rows, s, a);
 }
 
 }  // namespace

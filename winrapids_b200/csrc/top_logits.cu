@@ -178,8 +178,8 @@ cudaError_t launch(const TopArgs& a, int num_sms, cudaStream_t s) {
   constexpr int NT = 512;
   const int c = cluster_size(bytes, NT * NV * 16, a.x.rows, num_sms, NT);
   const bool res = static_cast<long long>(c) * NT * NV * 16 >= bytes + 32;
-  if (res) return launch_rows(top_logits_kernel<T, NT, true>, NT, c, 0, a, a.x.rows, s);
-  return launch_rows(top_logits_kernel<T, NT, false>, NT, c, 0, a, a.x.rows, s);
+  if (res) return launch_rows(top_logits_kernel<T, NT, true>, NT, c, 0, a.x.rows, s, a);
+  return launch_rows(top_logits_kernel<T, NT, false>, NT, c, 0, a.x.rows, s, a);
 }
 
 }  // namespace
