@@ -6,6 +6,7 @@
 #include <climits>
 
 #include "logits_select.cuh"
+#include "logits_stream.cuh"
 
 namespace tbgb {
 
@@ -13,24 +14,30 @@ namespace {
 
 using namespace row;
 
-template <typename T, int NT, bool RES>
-__global__ void __launch_bounds__(NT) top_logits_kernel(const TopArgs a) {
-  __shared__ SelectSmem sel;
-  __shared__ unsigned long long list[kTopMax];
-  __shared__ int n_list;
-  __shared__ float wm[NT / 32], ws[NT / 32];
-  __shared__ float2 cta_ms;
-  __shared__ int warp_ties[NT / 32], cta_ties;
+struct ExactSmem {
+  SelectSmem sel;
+  unsigned long long list[kTopMax];
+  float wm[32], ws[32];
+  float2 cta_ms;
+  int warp_ties[32], cta_ties, n_list;
+};
+
+// A row by radix descent over the keys and the ids' order: right for any number of equal logits, NaN and
+// infinities, at several passes over the row.  For rows that do not fit the lists below.
+template <typename T, int NT>
+__device__ __noinline__ void exact_row(const TopArgs& a, long long r, ExactSmem& sm) {
+  constexpr bool RES = false;
+  SelectSmem& sel = sm.sel;
+  unsigned long long* list = sm.list;
+  int& n_list = sm.n_list;
+  float *wm = sm.wm, *ws = sm.ws;
+  float2& cta_ms = sm.cta_ms;
+  int *warp_ties = sm.warp_ties, &cta_ties = sm.cta_ties;
   cg::cluster_group cl = cg::this_cluster();
   const int C = static_cast<int>(cl.num_blocks()), rank = static_cast<int>(cl.block_rank());
-  const long long r = blockIdx.x / C;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   Slice<T, NT, RES> sl(static_cast<const T*>(a.x.logits) + r * a.x.ld, a.x.vocab,
                        a.mask ? a.mask + r * a.mask_ld : nullptr, rank, C);
-  if (RES) {
-    sl.load(0);
-    sl.clean(0);
-  }
   if (tid == 0) n_list = 0;
 
   // log-sum-exp
@@ -172,14 +179,118 @@ __global__ void __launch_bounds__(NT) top_logits_kernel(const TopArgs a) {
   }
 }
 
+// One cluster per row: the pass of collect_top carries the running maximum and sum of the softmax too,
+// so the row is read once from HBM.
+template <typename T, int NT, bool MASK>
+__global__ void __launch_bounds__(NT, 1024 / NT) top_logits_kernel(const TopArgs a) {
+  extern __shared__ __align__(16) char dyn[];
+  __shared__ TopSmem sm;
+  __shared__ float2 w_ms[NT / 32], cta_ms;
+  cg::cluster_group cl = cg::this_cluster();
+  const int C = static_cast<int>(cl.num_blocks()), rank = static_cast<int>(cl.block_rank());
+  const long long r = blockIdx.x / C;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  TopLists li;
+  li.vec_cap = top_vec_cap(a.k);
+  li.el_cap = top_el_cap(a.k);
+  li.el = reinterpret_cast<unsigned long long*>(dyn);
+  li.vec = li.el + li.el_cap;
+  const Stream<T, NT, MASK> st(static_cast<const T*>(a.x.logits) + r * a.x.ld, a.x.vocab,
+                               MASK ? a.mask + r * a.mask_ld : nullptr, rank, C);
+  const float scale = 1.4426950408889634f / a.temperature;
+  const float2 scale2 = make_float2(scale, scale);
+  const bool with_lse = a.lse != nullptr;
+  float m = neg_inff();
+  float2 sum = make_float2(0.0f, 0.0f);
+  collect_top<T, NT, MASK>(st, a.k, sm, li, [&](const uint4 (&x)[STEP], float top) {
+    if (!with_lse) return;
+    if (top > m) {  // the sum is scaled when the maximum rises
+      const float f = m == neg_inff() ? 1.0f : power2((m - top) * scale);
+      sum = mul2(sum, make_float2(f, f));
+      m = top;
+    }
+    const float ref = m == neg_inff() ? 0.0f : m;
+    const float2 minus_ref = make_float2(-ref, -ref);
+#pragma unroll
+    for (int i = 0; i < STEP; ++i)
+#pragma unroll
+      for (int j = 0; j < Elem<T>::PAIRS; ++j) sum = add2(sum, power2(Elem<T>::pair(x[i], j), minus_ref, scale2));
+  });
+  if (with_lse) {
+    const float m_w = warp_max(m);
+    const float s_w = warp_sum(m == neg_inff() || m == m_w ? sum.x + sum.y : (sum.x + sum.y) * power2((m - m_w) * scale));
+    if (lane == 0) w_ms[warp] = make_float2(m_w, s_w);
+    __syncthreads();
+    if (tid == 0) {
+      MaxSum ms{neg_inff(), 0.0f};
+      for (int w = 0; w < NT / 32; ++w) ms.merge(w_ms[w].x, w_ms[w].y, scale);
+      cta_ms = make_float2(ms.m, ms.s);
+      if (!(ms.s < -neg_inff())) sm.spilled = 1;  // a NaN or an infinity: the exact row leaves NaN out
+    }
+  }
+  cl.sync();
+  bool any = false;
+  int n = 0;
+  for (int c = 0; c < C; ++c) {
+    const TopSmem* peer = cl.map_shared_rank(&sm, c);
+    any |= peer->spilled != 0;
+    n += peer->n_el;
+  }
+  any |= n > li.el_cap;
+  if (any) {  // the same for every CTA of the cluster
+    cl.sync();
+    exact_row<T, NT>(a, r, *reinterpret_cast<ExactSmem*>(dyn));
+    return;
+  }
+  if (rank == 0) {
+    if (with_lse && tid == 0) {
+      MaxSum ms{neg_inff(), 0.0f};
+      for (int c = 0; c < C; ++c) {
+        const float2 p = *cl.map_shared_rank(&cta_ms, c);
+        ms.merge(p.x, p.y, scale);
+      }
+      a.lse[r] = ms.m == neg_inff() ? neg_inff() : ms.m / a.temperature + logf(ms.s);
+    }
+    int at = sm.n_el;
+    for (int c = 1; c < C; ++c) {
+      const int nc = cl.map_shared_rank(&sm, c)->n_el;
+      const unsigned long long* src = cl.map_shared_rank(li.el, c);
+      for (int j = tid; j < nc; j += NT) li.el[at + j] = src[j];
+      at += nc;
+    }
+  }
+  if (C > 1) cl.sync();  // the lists have been read
+  if (rank != 0) return;
+  __syncthreads();
+  sort_list<NT>(li.el, n);
+  for (int j = tid; j < a.k; j += NT) {
+    const bool have = j < n;
+    const long long o = r * a.k + j;
+    const unsigned long long u = have ? li.el[j] : 0;
+    a.ids[o] = have ? static_cast<int>(~static_cast<uint32_t>(u)) : -1;
+    const uint32_t bits = have ? Elem<T>::to_bits(Elem<float>::unkey(static_cast<uint32_t>(u >> 32))) : Elem<T>::NEG_INF;
+    if (sizeof(T) == 4)
+      static_cast<uint32_t*>(a.values)[o] = bits;
+    else
+      static_cast<unsigned short*>(a.values)[o] = static_cast<unsigned short>(bits);
+  }
+}
+
 template <typename T>
 cudaError_t launch(const TopArgs& a, int num_sms, cudaStream_t s) {
-  const long long bytes = static_cast<long long>(a.x.vocab) * sizeof(T);
   constexpr int NT = 512;
-  const int c = cluster_size(bytes, NT * NV * 16, a.x.rows, num_sms, NT);
-  const bool res = static_cast<long long>(c) * NT * NV * 16 >= bytes + 32;
-  if (res) return launch_rows(top_logits_kernel<T, NT, true>, NT, c, 0, a.x.rows, s, a);
-  return launch_rows(top_logits_kernel<T, NT, false>, NT, c, 0, a.x.rows, s, a);
+  const long long nvec = static_cast<long long>(a.x.vocab) * sizeof(T) / 16 + 2;
+  // more CTAs for a row while rows leave SMs without work, a lane keeps a step and the lists hold them all
+  int c = 1;
+  while (c < 8 && a.x.rows * c * 2 <= num_sms && nvec / (c * 2) >= NT && c * 2 * a.k * 5 / 4 + 64 < top_el_cap(a.k)) c *= 2;
+  const size_t lists = (static_cast<size_t>(top_vec_cap(a.k)) + top_el_cap(a.k)) * 8;
+  const size_t smem = lists > sizeof(ExactSmem) ? lists : sizeof(ExactSmem);
+  auto kernel = a.mask ? top_logits_kernel<T, NT, true> : top_logits_kernel<T, NT, false>;
+  if (smem > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (e != cudaSuccess) return e;
+  }
+  return launch_rows(kernel, NT, c, smem, a.x.rows, s, a);
 }
 
 }  // namespace
