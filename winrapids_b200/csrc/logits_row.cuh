@@ -26,6 +26,12 @@ constexpr unsigned FULL = 0xffffffffu;
 
 __device__ __forceinline__ float neg_inff() { return __uint_as_float(0xff800000u); }
 
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // ---- element types -------------------------------------------------------------------------
 // KEY_BITS-bit ordered keys: k(a) < k(b) iff a < b, equal zeros, -inf lowest (NaN is replaced
 // by -inf before keys are taken).
@@ -54,6 +60,9 @@ struct Elem<float> {
   }
   static __device__ __forceinline__ float vmax(const uint4& v) {
     return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
+  }
+  static __device__ __forceinline__ float vmax_nan(const uint4& v) {  // NaN when one is among them
+    return max_nan(max_nan(__uint_as_float(v.x), __uint_as_float(v.y)), max_nan(__uint_as_float(v.z), __uint_as_float(v.w)));
   }
   static __device__ __forceinline__ uint32_t load_bits(const float* p) { return __float_as_uint(*p); }
   static __device__ __forceinline__ float from_bits(uint32_t b) { return __uint_as_float(b); }
@@ -107,6 +116,10 @@ struct Elem<__nv_bfloat16> : Elem16<__nv_bfloat16> {
     const __nv_bfloat162 h = __floats2bfloat162_rn(f.x, f.y);
     (i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w) = *reinterpret_cast<const uint32_t*>(&h);
   }
+  static __device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b) {
+    const __nv_bfloat162 h = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
   static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
     const __nv_bfloat162 h = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -114,6 +127,10 @@ struct Elem<__nv_bfloat16> : Elem16<__nv_bfloat16> {
   static __device__ __forceinline__ float vmax(const uint4& v) {
     const uint32_t m = max2(max2(v.x, v.y), max2(v.z, v.w));
     return fmaxf(__uint_as_float(m << 16), __uint_as_float(m & 0xffff0000u));
+  }
+  static __device__ __forceinline__ float vmax_nan(const uint4& v) {
+    const uint32_t m = max2_nan(max2_nan(v.x, v.y), max2_nan(v.z, v.w));
+    return max_nan(__uint_as_float(m << 16), __uint_as_float(m & 0xffff0000u));
   }
   static __device__ __forceinline__ float from_bits(uint32_t b) { return __uint_as_float(b << 16); }
   static __device__ __forceinline__ uint32_t to_bits(float f) {
@@ -143,6 +160,10 @@ struct Elem<__half> : Elem16<__half> {
     const __half2 h = __floats2half2_rn(f.x, f.y);
     (i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w) = *reinterpret_cast<const uint32_t*>(&h);
   }
+  static __device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b) {
+    const __half2 h = __hmax2_nan(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
   static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
     const __half2 h = __hmax2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -151,6 +172,11 @@ struct Elem<__half> : Elem16<__half> {
     const uint32_t m = max2(max2(v.x, v.y), max2(v.z, v.w));
     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&m));
     return fmaxf(f.x, f.y);
+  }
+  static __device__ __forceinline__ float vmax_nan(const uint4& v) {
+    const uint32_t m = max2_nan(max2_nan(v.x, v.y), max2_nan(v.z, v.w));
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&m));
+    return max_nan(f.x, f.y);
   }
   static __device__ __forceinline__ float get(const uint4& v, int e) {
     const uint32_t w = word(v, e >> 1);

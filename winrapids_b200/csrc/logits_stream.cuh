@@ -154,27 +154,21 @@ __host__ __device__ inline int top_el_cap(int k) { return k <= 256 ? 1024 : 4096
 // Fills lists.el (sm.n_el entries) with every element of the CTA's slice that is not below the returned bound;
 // the K largest of the slice are among them.  sm.spilled is set when the lists are too short (many equal
 // elements).  With `pass` the caller sees every step of the pass over the slice too (x, base).
-//   1. a sample (the first steps of every warp, a quarter of the row at 131072 16-bit logits): the K-th largest
+//   1. a sample (the first 4096 vectors of the warps' parts, a quarter of the row at 131072 16-bit logits): the K-th largest
 //      of its lanes' (for many K its vectors') maxima is a first bound
 //   2. one pass: vectors whose maximum reaches it are listed
 //   3. the K-th largest of the listed maxima is the bound: their elements above it are listed
 template <typename T, int NT, bool MASK, typename F>
 __device__ __forceinline__ void collect_top(const Stream<T, NT, MASK>& st, int K, TopSmem& sm, const TopLists& li, F pass) {
-  constexpr int SAMPLE = 2 * 32 * STEP;
+  constexpr int SAMPLE = 4096 / NT;  // vectors of a lane
   const int tid = threadIdx.x, lane = tid & 31;
-  float s[2 * STEP], most = neg_inff();
+  float s[SAMPLE], most = neg_inff();
 #pragma unroll
-  for (int i = 0; i < 2 * STEP; ++i) s[i] = neg_inff();
-#pragma unroll
-  for (int g = 0; g < 2; ++g) {
-#pragma unroll
-    for (int i = 0; i < STEP; ++i) {
-      const int v = st.a + (g * STEP + i) * 32 + lane;
-      if (v < st.b) s[g * STEP + i] = Elem<T>::vmax(st.load(v));
-      most = fmaxf(most, s[g * STEP + i]);
-    }
+  for (int i = 0; i < SAMPLE; ++i) {
+    const int v = st.a + i * 32 + lane;
+    s[i] = v < st.b ? Elem<T>::vmax(st.load(v)) : neg_inff();
+    most = fmaxf(most, s[i]);
   }
-  (void)SAMPLE;
   if (tid == 0) sm.n_vec = sm.n_el = sm.spilled = 0;
   const bool lanes_do = K <= NT / 4;
   const float tau0 = kth_bound<NT>(sm.bound, K, [&](auto g) {
@@ -182,7 +176,7 @@ __device__ __forceinline__ void collect_top(const Stream<T, NT, MASK>& st, int K
       if (most > neg_inff()) g(most);
     } else {
 #pragma unroll
-      for (int i = 0; i < 2 * STEP; ++i)
+      for (int i = 0; i < SAMPLE; ++i)
         if (s[i] > neg_inff()) g(s[i]);
     }
   });

@@ -13,9 +13,11 @@
 // Each cut keeps a prefix of the same order, so all of them together are one threshold: a key tau
 // and how many of the tokens equal to it are kept (the lowest ids).  The token is the first, in the
 // order of the ids, whose running sum exceeds floor(u W'), W' the sum of what is kept.
+#include <algorithm>
 #include <climits>
 
 #include "logits_select.cuh"
+#include "logits_stream.cuh"
 
 namespace tbgb {
 
@@ -38,24 +40,30 @@ struct Share {  // one CTA's part of what is kept
   unsigned ties;            // tokens at tau
 };
 
-template <typename T, int NT, bool RES>
-__global__ void __launch_bounds__(NT) sample_kernel(const SampleArgs a) {
+struct ExactSmem {
+  SelectSmem sel;
+  float wm[32], cta_max;
+  unsigned long long w_sure[32], cta_sum;
+  unsigned w_ties[32];
+  Share share;
+};
+
+// A row by radix descent and passes over all of it: right for any number of equal logits, NaN, infinities, any
+// temperature and any k.  For rows that the quicker ways below do not take.
+template <typename T, int NT>
+__device__ __noinline__ void exact_row(const SampleArgs& a, long long r, ExactSmem& sm) {
   constexpr int NW = NT / 32;
-  __shared__ SelectSmem sel;
-  __shared__ float wm[NW], cta_max;
-  __shared__ unsigned long long w_sure[NW], cta_sum;
-  __shared__ unsigned w_ties[NW];
-  __shared__ Share share;
+  constexpr bool RES = false;
+  SelectSmem& sel = sm.sel;
+  float *wm = sm.wm, &cta_max = sm.cta_max;
+  unsigned long long *w_sure = sm.w_sure, &cta_sum = sm.cta_sum;
+  unsigned* w_ties = sm.w_ties;
+  Share& share = sm.share;
   cg::cluster_group cl = cg::this_cluster();
   const int C = static_cast<int>(cl.num_blocks()), rank = static_cast<int>(cl.block_rank());
-  const long long r = blockIdx.x / C;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   Slice<T, NT, RES> sl(static_cast<const T*>(a.x.logits) + r * a.x.ld, a.x.vocab,
                        a.mask ? a.mask + r * a.mask_ld : nullptr, rank, C);
-  if (RES) {
-    sl.load(0);
-    sl.clean(0);
-  }
   const float temperature = a.p.temperature ? a.p.temperature[r] : a.p.temperature_all;
   const int top_k = a.p.top_k ? a.p.top_k[r] : a.p.top_k_all;
   const float top_p = a.p.top_p ? a.p.top_p[r] : a.p.top_p_all;
@@ -269,14 +277,548 @@ __global__ void __launch_bounds__(NT) sample_kernel(const SampleArgs a) {
   }
 }
 
+// ---- the quick ways ------------------------------------------------------------------------------------
+//
+// A kept prefix is all tokens whose (key of the logit, ~id), as one whole number, is at least `cut`: ties need no
+// counting.
+//   top-k (k <= 1024), greedy   the k largest are collected in one pass (logits_stream.cuh); everything
+//                               else happens in that sorted list
+//   nothing but min-p           a pass for the largest logit, one for the weights, summed per warp
+//   top-p                       a pass for the largest logit, one for the sum W; one that counts the weights into
+//                               1024 equal parts of the exponent's range, which finds the part that holds the
+//                               prefix's end; one that lists that part and sums what lies above it
+// The first pass reads HBM, the others L2.  Weights below 2^-7 are turned into whole numbers by an addition:
+// 2^-7 + e has steps of 2^-30, so its bits less those of 2^-7 are e in those units (rounded to nearest,
+// ties to even, as the conversion does), and bits are summed.  A conversion would cost a second
+// instruction on the special function units, which are busy for most of the pass with the power itself.
+
+constexpr int kParts = 1024;       // of the exponent's range
+// Tokens of the part that holds the end of the prefix: equal 16-bit logits between 16 and 32 are up to one in 30 of a
+// vocabulary with a spread of 2.
+constexpr int kEdgeMost = 4096;
+constexpr float kSmall = 0.0078125f;  // 2^-7
+
+struct SampleSmem {
+  TopSmem top;
+  float f[32];
+  unsigned long long w[32];
+  unsigned long long cta_w, above, cut;
+  float cta_f;
+  int n_edge, part;
+  unsigned long long sub[32];
+};
+
+template <typename T, int NT, bool MASK>
+struct Sampler {
+  static constexpr int NW = NT / 32, EPV = Elem<T>::EPV, PAIRS = Elem<T>::PAIRS;
+  const SampleArgs& a;
+  const Stream<T, NT, MASK>& st;
+  SampleSmem& sm;
+  cg::cluster_group& cl;
+  long long r;
+  int C, rank;
+  float temperature, min_p;
+  Weight weight;
+
+  __device__ __forceinline__ unsigned long long order_key(float z, int id) const {
+    return (static_cast<unsigned long long>(Elem<float>::key(z)) << 32) | static_cast<uint32_t>(~id);
+  }
+  // sum of a u64 over the cluster, the same in every thread; `own_before` the sum over the CTAs in front
+  __device__ __forceinline__ unsigned long long cluster_sum(unsigned long long warp_total, unsigned long long* own,
+                                                            unsigned long long* before) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if (lane == 0) sm.w[warp] = warp_total;
+    __syncthreads();
+    unsigned long long mine = warp_sum(lane < NW ? sm.w[lane] : 0ull);
+    *own = mine;
+    *before = 0;
+    if (C == 1) return mine;
+    if (threadIdx.x == 0) sm.cta_w = mine;
+    cl.sync();
+    unsigned long long all = 0;
+    for (int c = 0; c < C; ++c) {
+      const unsigned long long v = *cl.map_shared_rank(&sm.cta_w, c);
+      if (c < rank) *before += v;
+      all += v;
+    }
+    cl.sync();
+    return all;
+  }
+  // the weights of a vector's elements that pass keep(z, power, id), by conversion
+  template <typename K>
+  __device__ __forceinline__ unsigned long long exact_weights(const uint4& x, int v, K keep) const {
+    unsigned long long s = 0;
+#pragma unroll
+    for (int e = 0; e < EPV; ++e) {
+      const float z = Elem<T>::get(x, e);
+      const float p = z > neg_inff() ? weight.power(z) : 0.0f;
+      if (keep(z, p, st.index(v, e))) s += __float2uint_rn(p * kGrid);
+    }
+    return s;
+  }
+  // All weights of this warp's part, nothing cut off.
+  __device__ __forceinline__ unsigned long long all_weights() const {
+    unsigned long long s = 0;
+    const int lane = threadIdx.x & 31;
+    const float2 minus = make_float2(-weight.zmax, -weight.zmax), scale2 = make_float2(weight.scale, weight.scale),
+                 small2 = make_float2(kSmall, kSmall);
+    st.each(st.a, st.b, [&](const uint4 (&x)[STEP], int base) {
+      unsigned bits = 0;
+#pragma unroll
+      for (int i = 0; i < STEP; ++i) {
+        if ((Elem<T>::vmax(x[i]) - weight.zmax) * weight.scale < -7.0f) {
+#pragma unroll
+          for (int j = 0; j < PAIRS; ++j) {
+            const float2 q = add2(power2(Elem<T>::pair(x[i], j), minus, scale2), small2);
+            bits += __float_as_uint(q.x) + __float_as_uint(q.y);
+          }
+          bits -= static_cast<unsigned>(EPV) * __float_as_uint(kSmall);  // (modulo 2^32: what is left is below it)
+        } else {
+          s += exact_weights(x[i], base + 32 * i + lane, [](float, float, int) { return true; });
+        }
+      }
+      s += bits;
+    });
+    return s;
+  }
+  // Weights of [from, to) that pass keep(z, power, id); vectors whose largest logit is below `least` have none.
+  template <typename K>
+  __device__ __forceinline__ unsigned long long kept_weights(int from, int to, float least, K keep) const {
+    unsigned long long s = 0;
+    const int lane = threadIdx.x & 31;
+    st.each(from, to, [&](const uint4 (&x)[STEP], int base) {
+#pragma unroll 1
+      for (int i = 0; i < STEP; ++i) {
+        const uint4 y = i == 0 ? x[0] : i == 1 ? x[1] : i == 2 ? x[2] : x[3];
+        if (Elem<T>::vmax(y) >= least) s += exact_weights(y, base + 32 * i + lane, keep);
+      }
+    });
+    return s;
+  }
+  __device__ __forceinline__ float logprob(float z, unsigned long long total) const {
+    return (z == weight.zmax ? 0.0f : (z - weight.zmax) / temperature) -
+           logf(static_cast<float>(static_cast<double>(total) / kGrid));
+  }
+  __device__ __forceinline__ unsigned long long target_of(unsigned long long total) const {
+    const double goal = floor(static_cast<double>(a.u[r]) * static_cast<double>(total));
+    unsigned long long t = goal > 0.0 ? static_cast<unsigned long long>(goal) : 0ull;
+    return t >= total ? total - 1 : t;
+  }
+  // The token, from the warps' sums of kept weights (sm.w, this CTA's from `before` on).
+  template <typename K>
+  __device__ __forceinline__ void pick(unsigned long long total, unsigned long long own, unsigned long long before,
+                                       float least, K keep) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    unsigned long long target = target_of(total);
+    if (target < before || target >= before + own) return;
+    target -= before;
+    const unsigned long long part = lane < NW ? sm.w[lane] : 0;
+    const unsigned long long upto = warp_inclusive(part);
+    int at = __ffs(__ballot_sync(FULL, upto > target)) - 1;  // the warp whose part holds the token
+    target -= __shfl_sync(FULL, upto - part, at);
+    // all warps share that part
+    const int per = ((st.v1 - st.v0 + NT - 1) / NT) * 32;
+    const int from = min(st.v0 + at * per, st.v1), to = min(from + per, st.v1);
+    const int each = ((to - from + NT - 1) / NT) * 32;
+    const int f = min(from + warp * each, to), t = min(f + each, to);
+    const unsigned long long mine = warp_sum(kept_weights(f, t, least, keep));
+    if (lane == 0) sm.sub[warp] = mine;
+    __syncthreads();
+    const unsigned long long p2 = lane < NW ? sm.sub[lane] : 0;
+    const unsigned long long u2 = warp_inclusive(p2);
+    at = __ffs(__ballot_sync(FULL, u2 > target)) - 1;
+    if (warp != at) return;
+    target -= __shfl_sync(FULL, u2 - p2, at);
+    for (int v0 = f; v0 < t; v0 += 32) {
+      const int v = v0 + lane;
+      uint4 x = RowView<T>::none();
+      if (v < t) x = st.load(v);
+      const unsigned long long s = v < t && Elem<T>::vmax(x) >= least ? exact_weights(x, v, keep) : 0;
+      const unsigned long long inc = warp_inclusive(s);
+      const unsigned long long all = __shfl_sync(FULL, inc, 31);
+      if (target >= all) {
+        target -= all;
+        continue;
+      }
+      if (target >= inc - s && target < inc) {
+        unsigned long long left = target - (inc - s);
+#pragma unroll 1
+        for (int e = 0; e < EPV; ++e) {
+          const int id = st.index(v, e);
+          if (id < 0 || id >= a.x.vocab) continue;
+          float z = neg_inff();
+#pragma unroll
+          for (int k = 0; k < EPV; ++k)
+            if (k == e) z = Elem<T>::get(x, k);
+          const float p = z > neg_inff() ? weight.power(z) : 0.0f;
+          const unsigned long long w = keep(z, p, id) ? __float2uint_rn(p * kGrid) : 0u;
+          if (left < w) {
+            a.tokens[r] = id;
+            if (a.logprobs) a.logprobs[r] = logprob(z, total);
+            break;
+          }
+          left -= w;
+        }
+      }
+      break;
+    }
+  }
+};
+
+template <typename T, int NT, bool MASK>
+__global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs a, int list_k) {
+  constexpr int NW = NT / 32;
+  extern __shared__ __align__(16) char dyn[];
+  __shared__ SampleSmem sm;
+  cg::cluster_group cl = cg::this_cluster();
+  const int C = static_cast<int>(cl.num_blocks()), rank = static_cast<int>(cl.block_rank());
+  const long long r = blockIdx.x / C;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const float temperature = a.p.temperature ? a.p.temperature[r] : a.p.temperature_all;
+  const int top_k = a.p.top_k ? a.p.top_k[r] : a.p.top_k_all;
+  const float top_p = a.p.top_p ? a.p.top_p[r] : a.p.top_p_all;
+  const float min_p = fminf(a.p.min_p ? a.p.min_p[r] : a.p.min_p_all, 1.0f);  // the largest logit always stays
+  const Stream<T, NT, MASK> st(static_cast<const T*>(a.x.logits) + r * a.x.ld, a.x.vocab,
+                               MASK ? a.mask + r * a.mask_ld : nullptr, rank, C);
+  const bool greedy = !(temperature > 0.0f);
+  const int k = greedy ? 1 : top_k;
+  auto exact = [&]() {
+    cl.sync();  // every CTA of the cluster is done with what lies there
+    exact_row<T, NT>(a, r, *reinterpret_cast<ExactSmem*>(dyn));
+  };
+
+  if (k > 0 && k <= list_k) {
+    // ---- the k largest in a list
+    TopLists li;
+    li.vec_cap = top_vec_cap(list_k);
+    li.el_cap = top_el_cap(list_k);
+    li.el = reinterpret_cast<unsigned long long*>(dyn);
+    li.vec = li.el + li.el_cap;
+    collect_top<T, NT, MASK>(st, k, sm.top, li, [](const uint4 (&)[STEP], float) {});
+    if (C > 1) cl.sync();
+    else __syncthreads();
+    bool any = false;
+    int n = 0;
+    for (int c = 0; c < C; ++c) {
+      const TopSmem* peer = cl.map_shared_rank(&sm.top, c);
+      any |= peer->spilled != 0;
+      n += peer->n_el;
+    }
+    if (any || n > li.el_cap) {
+      exact();
+      return;
+    }
+    if (rank == 0) {
+      int at = sm.top.n_el;
+      for (int c = 1; c < C; ++c) {
+        const int nc = cl.map_shared_rank(&sm.top, c)->n_el;
+        const unsigned long long* src = cl.map_shared_rank(li.el, c);
+        for (int j = tid; j < nc; j += NT) li.el[at + j] = src[j];
+        at += nc;
+      }
+    }
+    if (C > 1) cl.sync();  // the lists have been read
+    if (rank != 0) return;
+    __syncthreads();
+    sort_list<NT>(li.el, n);
+    n = min(n, k);
+    if (n == 0 || greedy) {
+      if (tid == 0) {
+        a.tokens[r] = n ? static_cast<int>(~static_cast<uint32_t>(li.el[0])) : -1;
+        if (a.logprobs) a.logprobs[r] = n ? 0.0f : neg_inff();
+      }
+      return;
+    }
+    const Weight weight{Elem<float>::unkey(static_cast<uint32_t>(li.el[0] >> 32)), 1.4426950408889634f / temperature};
+    auto z_of = [&](int j) { return Elem<float>::unkey(static_cast<uint32_t>(li.el[j] >> 32)); };
+    // running sums by warp 0, in chunks of 32: top-p, then what min-p leaves, as (~id, weight) for the second sort
+    if (warp == 0) {
+      unsigned long long W = 0;
+      for (int j = lane; j < n; j += 32) W += weight.unit(z_of(j));
+      W = warp_sum(W);
+      unsigned long long need = ~0ull;
+      if (top_p < 1.0f) {
+        const double want = ceil(static_cast<double>(top_p) * static_cast<double>(W));
+        need = want >= 1.0 ? static_cast<unsigned long long>(want) : 1ull;
+      }
+      unsigned long long run = 0;
+      int kept = 0;
+      for (int j0 = 0; j0 < n; j0 += 32) {
+        const int j = j0 + lane;
+        const float z = j < n ? z_of(j) : neg_inff();
+        const float e = j < n ? weight.power(z) : 0.0f;
+        const unsigned w = j < n ? __float2uint_rn(e * kGrid) : 0u;
+        const unsigned long long inc = warp_inclusive(static_cast<unsigned long long>(w));
+        const bool keep = j < n && run + inc - w < need && e >= min_p;
+        if (keep) li.vec[j] = (li.el[j] << 32) | w;  // ~id in the upper half: larger for lower ids
+        kept += __popc(__ballot_sync(FULL, keep));  // a prefix
+        run += __shfl_sync(FULL, inc, 31);
+      }
+      if (lane == 0) sm.n_edge = kept;
+    }
+    __syncthreads();
+    n = sm.n_edge;
+    sort_list<NT>(li.vec, n);
+    if (warp == 0) {
+      unsigned long long W = 0;
+      for (int j = lane; j < n; j += 32) W += static_cast<uint32_t>(li.vec[j]);
+      W = warp_sum(W);
+      const double goal = floor(static_cast<double>(a.u[r]) * static_cast<double>(W));
+      unsigned long long target = goal > 0.0 ? static_cast<unsigned long long>(goal) : 0ull;
+      if (target >= W) target = W - 1;
+      unsigned long long run = 0;
+      for (int j0 = 0; j0 < n; j0 += 32) {
+        const int j = j0 + lane;
+        const unsigned long long w = j < n ? static_cast<uint32_t>(li.vec[j]) : 0;
+        const unsigned long long inc = run + warp_inclusive(w);
+        if (target < inc && target >= inc - w) {
+          const int id = static_cast<int>(~static_cast<uint32_t>(li.vec[j] >> 32));
+          a.tokens[r] = id;
+          if (a.logprobs) {
+            const T* p = static_cast<const T*>(a.x.logits) + r * a.x.ld + id;
+            const float z = Elem<T>::from_bits(Elem<T>::load_bits(p));
+            a.logprobs[r] = (z == weight.zmax ? 0.0f : (z - weight.zmax) / temperature) -
+                            logf(static_cast<float>(static_cast<double>(W) / kGrid));
+          }
+        }
+        run = __shfl_sync(FULL, inc, 31);
+      }
+    }
+    return;
+  }
+
+  // ---- the largest logit
+  float m = neg_inff();
+  st.each(st.a, st.b, [&](const uint4 (&x)[STEP], int) {
+#pragma unroll
+    for (int i = 0; i < STEP; ++i) m = max_nan(m, Elem<T>::vmax_nan(x[i]));
+  });
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(FULL, m, o));
+  if (lane == 0) sm.f[warp] = m;
+  __syncthreads();
+  m = sm.f[0];
+  for (int w = 1; w < NW; ++w) m = max_nan(m, sm.f[w]);
+  if (C > 1) {
+    if (tid == 0) sm.cta_f = m;
+    cl.sync();
+    for (int c = 0; c < C; ++c) m = max_nan(m, *cl.map_shared_rank(&sm.cta_f, c));
+    cl.sync();
+  }
+  if (m == neg_inff()) {  // nothing is allowed (the same for every CTA of the cluster)
+    if (rank == 0 && tid == 0) {
+      a.tokens[r] = -1;
+      if (a.logprobs) a.logprobs[r] = neg_inff();
+    }
+    return;
+  }
+  const float scale = 1.4426950408889634f / temperature;
+  // NaN, infinite logits, an infinite temperature, many more than the lists hold: the exact row
+  const bool cut_p = top_p < 1.0f;
+  if (!(m <= 3.402823466e38f) || !(scale > 0.0f) || (top_k > 0 && top_k < a.x.vocab) ||
+      (cut_p && a.x.vocab / C > 131072)) {
+    exact();
+    return;
+  }
+  Sampler<T, NT, MASK> sp{a, st, sm, cl, r, C, rank, temperature, min_p, Weight{m, scale}};
+  unsigned long long own, before;
+  // no vector below this logit has a token with a power of min_p: d < log2(min_p) by more than any rounding
+  const float floor_d = min_p > 0.0f ? log2f(min_p) - 0.01f : -40.0f;
+  const float reach = floor_d / scale;
+  float least = m + (reach - fabsf(reach) * 1e-5f) - fabsf(m) * 1e-6f;
+  if (!cut_p) {
+    if (min_p > 0.0f) {
+      auto keep = [&](float, float p, int) { return p >= min_p; };
+      const unsigned long long mine = warp_sum(sp.kept_weights(st.a, st.b, least, keep));
+      const unsigned long long total = sp.cluster_sum(mine, &own, &before);
+      sp.pick(total, own, before, least, keep);
+    } else {
+      auto keep = [](float, float, int) { return true; };
+      const unsigned long long total = sp.cluster_sum(warp_sum(sp.all_weights()), &own, &before);
+      sp.pick(total, own, before, least, keep);
+    }
+    return;
+  }
+
+  // ---- top-p
+  const unsigned long long W = sp.cluster_sum(warp_sum(sp.all_weights()), &own, &before);
+  const double want = ceil(static_cast<double>(top_p) * static_cast<double>(W));
+  const unsigned long long need = want >= 1.0 ? static_cast<unsigned long long>(want) : 1ull;
+  // tokens below (W - need) / V together weigh no more than W - need: the prefix ends above them
+  const float light = static_cast<float>(static_cast<double>(W - need) / a.x.vocab) * (1.0f / kGrid);
+  const float depth = fminf(31.5f, light > 1e-12f ? 0.01f - log2f(light) : 31.5f);
+  const float part_scale = kParts / depth;
+  auto part_of = [&](float z) {  // of a token: kParts and more lie below
+    const float d = z == m ? 0.0f : (z - m) * scale;
+    return static_cast<int>(fminf(-d * part_scale, 2.0f * kParts));
+  };
+  unsigned* lo = reinterpret_cast<unsigned*>(dyn);
+  unsigned* hi = lo + kParts;
+  unsigned long long* list = reinterpret_cast<unsigned long long*>(hi + kParts);
+  for (int i = tid; i < 2 * kParts; i += NT) lo[i] = 0;
+  if (tid == 0) sm.n_edge = 0;
+  __syncthreads();
+  float low = m - (depth / scale) * 1.00001f - fabsf(m) * 1e-6f;  // nothing below has a part
+  st.each(st.a, st.b, [&](const uint4 (&x)[STEP], int) {
+#pragma unroll 1
+    for (int i = 0; i < STEP; ++i) {
+      const uint4 y = i == 0 ? x[0] : i == 1 ? x[1] : i == 2 ? x[2] : x[3];
+      if (!(Elem<T>::vmax(y) >= low)) continue;
+#pragma unroll
+      for (int e = 0; e < Elem<T>::EPV; ++e) {
+        const float z = Elem<T>::get(y, e);
+        if (z >= low) {
+          const int b = part_of(z);
+          if (b < kParts) {
+            const unsigned w = sp.weight.unit(z);
+            atomicAdd(&lo[b], w & 32767u);  // 2^15 times 131072 tokens fit 32 bits
+            if (w >> 15) atomicAdd(&hi[b], w >> 15);
+          }
+        }
+      }
+    }
+  });
+  if (C > 1) cl.sync();
+  else __syncthreads();
+  // the cluster's sums of the parts (where the lists will be)
+  for (int b = tid; b < kParts; b += NT) {
+    unsigned long long v = 0;
+    for (int c = 0; c < C; ++c)
+      v += cl.map_shared_rank(lo, c)[b] + (static_cast<unsigned long long>(cl.map_shared_rank(hi, c)[b]) << 15);
+    list[b] = v;
+  }
+  __syncthreads();
+  if (warp == 0) {  // lane l takes parts 32 l, 32 l + 1, ...
+    unsigned long long sum = 0;
+    for (int j = 0; j < kParts / 32; ++j) sum += list[lane * (kParts / 32) + j];
+    const unsigned long long upto = warp_inclusive(sum);
+    const unsigned hit = __ballot_sync(FULL, upto >= need);
+    if (hit == 0) {
+      if (lane == 0) sm.part = -1;
+    } else if (lane == __ffs(hit) - 1) {
+      unsigned long long run = upto - sum;
+      int b = lane * (kParts / 32);
+      while (run + list[b] < need) run += list[b++];
+      sm.part = b;
+      sm.above = run;
+    }
+  }
+  if (C > 1) cl.sync();
+  else __syncthreads();
+  const int part = sm.part;
+  const unsigned long long above = sm.above;
+  if (part < 0) {
+    exact();
+    return;
+  }
+  // what lies above that part, per warp, and the part's own tokens
+  float edge = m - ((part + 1) / part_scale / scale) * 1.00001f - fabsf(m) * 1e-6f;
+  unsigned long long mine = 0;
+  st.each(st.a, st.b, [&](const uint4 (&x)[STEP], int base) {
+#pragma unroll 1
+    for (int i = 0; i < STEP; ++i) {
+      const uint4 y = i == 0 ? x[0] : i == 1 ? x[1] : i == 2 ? x[2] : x[3];
+      if (!(Elem<T>::vmax(y) >= edge)) continue;
+#pragma unroll
+      for (int e = 0; e < Elem<T>::EPV; ++e) {
+        const float z = Elem<T>::get(y, e);
+        if (z >= edge) {
+          const int b = part_of(z);
+          if (b < part) {
+            const float p = sp.weight.power(z);
+            if (p >= min_p) mine += __float2uint_rn(p * kGrid);
+          } else if (b == part) {
+            const int at = atomicAdd(&sm.n_edge, 1);
+            if (at < kEdgeMost) list[at] = sp.order_key(z, st.index(base + 32 * i + lane, e));
+          }
+        }
+      }
+    }
+  });
+  mine = warp_sum(mine);
+  if (C > 1) cl.sync();
+  else __syncthreads();
+  int n = 0;
+  for (int c = 0; c < C; ++c) n += *cl.map_shared_rank(&sm.n_edge, c);
+  if (n > kEdgeMost) {
+    exact();
+    return;
+  }
+  // the whole part, sorted, in every CTA (behind the CTA's own tokens): where the prefix ends
+  unsigned long long* all = C > 1 ? list + kEdgeMost : list;
+  int at = 0;
+  for (int c = 0; c < C && C > 1; ++c) {
+    const int nc = *cl.map_shared_rank(&sm.n_edge, c);
+    const unsigned long long* src = cl.map_shared_rank(list, c);
+    for (int j = tid; j < nc; j += NT) all[at + j] = src[j];
+    at += nc;
+  }
+  if (C > 1) cl.sync();
+  else __syncthreads();
+  sort_list<NT>(all, n);
+  if (warp == 0) {
+    unsigned long long run = above;
+    unsigned long long cut = 0;
+    for (int j0 = 0; j0 < n; j0 += 32) {
+      const int j = j0 + lane;
+      const unsigned long long w = j < n ? sp.weight.unit(Elem<float>::unkey(static_cast<uint32_t>(all[j] >> 32))) : 0;
+      const unsigned long long inc = run + warp_inclusive(w);
+      const unsigned hit = __ballot_sync(FULL, j < n && inc >= need);
+      if (hit) {
+        cut = all[j0 + __ffs(hit) - 1];
+        break;
+      }
+      run = __shfl_sync(FULL, inc, 31);
+    }
+    if (lane == 0) sm.cut = cut;
+  }
+  __syncthreads();
+  const unsigned long long cut = sm.cut;
+  auto keep = [&](float z, float p, int id) {
+    if (!(p >= min_p)) return false;
+    const int b = part_of(z);
+    return b < part || (b == part && sp.order_key(z, id) >= cut);
+  };
+  // kept tokens of the part go to their warps
+  const int per = ((st.v1 - st.v0 + NT - 1) / NT) * 32;
+  if (lane == 0) sm.sub[warp] = mine;
+  __syncthreads();
+  for (int j = tid; j < sm.n_edge; j += NT) {
+    const unsigned long long u = list[j];
+    const float z = Elem<float>::unkey(static_cast<uint32_t>(u >> 32));
+    const float p = sp.weight.power(z);
+    if (u >= cut && p >= min_p) {
+      const int id = static_cast<int>(~static_cast<uint32_t>(u));
+      const int v = (id + st.rv.off) / Elem<T>::EPV - st.v0;
+      atomicAdd(&sm.sub[v / per], static_cast<unsigned long long>(__float2uint_rn(p * kGrid)));
+    }
+  }
+  __syncthreads();
+  mine = sm.sub[warp];
+  const unsigned long long total = sp.cluster_sum(mine, &own, &before);
+  sp.pick(total, own, before, edge, keep);
+}
+
 template <typename T>
 cudaError_t launch(const SampleArgs& a, int num_sms, cudaStream_t s) {
-  const long long bytes = static_cast<long long>(a.x.vocab) * sizeof(T);
-  constexpr int NT = 512;
-  const int c = cluster_size(bytes, NT * NV * 16, a.x.rows, num_sms, NT);
-  const bool res = static_cast<long long>(c) * NT * NV * 16 >= bytes + 32;
-  if (res) return launch_rows(sample_kernel<T, NT, true>, NT, c, 0, a.x.rows, s, a);
-  return launch_rows(sample_kernel<T, NT, false>, NT, c, 0, a.x.rows, s, a);
+  constexpr int NT = 256;
+  const long long nvec = static_cast<long long>(a.x.vocab) * sizeof(T) / 16 + 2;
+  // the lists of the k largest: for the k of all rows where it is one, for 256 where rows have their own
+  const int k = a.p.top_k ? 256 : a.p.top_k_all;
+  const int list_k = k < 1 ? 1 : k > kTopMax ? kTopMax : k;
+  // more CTAs for a row while rows leave SMs without work, a lane keeps a step and the lists hold them all
+  int c = 1;
+  while (c < 8 && a.x.rows * c * 2 <= 2 * num_sms && nvec / (c * 2) >= NT && c * 2 * list_k * 5 / 4 + 64 < top_el_cap(list_k))
+    c *= 2;
+  size_t smem = (static_cast<size_t>(top_vec_cap(list_k)) + top_el_cap(list_k)) * 8;
+  smem = std::max(smem, sizeof(ExactSmem));
+  smem = std::max(smem, static_cast<size_t>(kParts) * 8 + (c > 1 ? 2 : 1) * kEdgeMost * 8);
+  auto kernel = a.mask ? sample_kernel<T, NT, true> : sample_kernel<T, NT, false>;
+  if (smem > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (e != cudaSuccess) return e;
+  }
+  return launch_rows(kernel, NT, c, smem, a.x.rows, s, a, list_k);
 }
 
 }  // namespace

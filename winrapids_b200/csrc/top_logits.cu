@@ -278,7 +278,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) top_logits_kernel(const TopArgs
 
 template <typename T>
 cudaError_t launch(const TopArgs& a, int num_sms, cudaStream_t s) {
-  constexpr int NT = 512;
+  constexpr int NT = 256;
   const long long nvec = static_cast<long long>(a.x.vocab) * sizeof(T) / 16 + 2;
   // more CTAs for a row while rows leave SMs without work, a lane keeps a step and the lists hold them all
   int c = 1;
