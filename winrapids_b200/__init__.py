@@ -33,10 +33,16 @@ __all__ = [
 SUMCOUNT_FIELDS = ("count", "sum", "mean")
 
 
-def _torch():
-    import torch
+_TORCH = None
 
-    return torch
+
+def _torch():
+    global _TORCH
+    if _TORCH is None:
+        import torch
+
+        _TORCH = torch
+    return _TORCH
 
 
 def _ptr(t) -> int | None:
@@ -53,6 +59,21 @@ def _stream_handle(stream) -> int | None:
     return int(getattr(stream, "cuda_stream", stream))
 
 
+_CODES: dict = {}
+
+
+def _logit_codes() -> dict:
+    """torch dtypes of logits -> tbgb_dtype."""
+    if not _CODES:
+        torch = _torch()
+        _CODES.update({torch.float32: DTYPES["f32"], torch.float16: DTYPES["f16"], torch.bfloat16: DTYPES["bf16"]})
+    return _CODES
+
+
+def _current_stream(device: int) -> int:
+    return _torch().cuda.current_stream(device).cuda_stream
+
+
 class Context:
     """One tbgb_ctx on one CUDA device."""
 
@@ -64,6 +85,7 @@ class Context:
             raise error_for(st, f"tbgb_create(device={device}) failed (an sm_100 device is required)")
         self._h = h
         self.device = int(device)
+        self._dev = _torch().device("cuda", self.device)
 
     def close(self):
         if getattr(self, "_h", None):
@@ -322,12 +344,12 @@ class Context:
     # stride, any alignment); token masks are row masks of the vocabulary, int64 [words] for every row
     # or [rows, words].
 
-    def _stream_scope(self, stream, *tensors):
-        """The handle of `stream` (None: torch's current one) and a scope in which new tensors belong to
-        it.  Tensors that come from another stream are kept until the work on `stream` is done."""
+    # These calls can be a few microseconds of device time: the checks below are kept short.
+
+    def _scope(self, stream, *tensors):
+        """The handle of `stream`, and a scope in which new tensors belong to it.  Tensors that come from
+        another stream are kept until the work on `stream` is done."""
         torch = _torch()
-        if stream is None:
-            return torch.cuda.current_stream(self.device).cuda_stream, contextlib.nullcontext()
         if not isinstance(stream, torch.cuda.Stream):
             stream = torch.cuda.ExternalStream(_stream_handle(stream), device=self.device)
         for t in tensors:
@@ -335,57 +357,53 @@ class Context:
                 t.record_stream(stream)
         return stream.cuda_stream, torch.cuda.stream(stream)
 
-    def _tensor(self, t, what: str, dtypes, shape=None):
+    def _check_tensor(self, t, what: str, dtypes):
         torch = _torch()
-        if not isinstance(t, torch.Tensor) or not t.is_cuda or t.device.index != self.device:
+        if not isinstance(t, torch.Tensor) or t.get_device() != self.device:
             raise InvalidArgument(7, f"{what} must be a tensor on cuda:{self.device}")
         if t.dtype not in dtypes:
             raise InvalidArgument(7, f"{what} has dtype {t.dtype}, not one of {', '.join(map(str, dtypes))}")
-        if shape is not None and tuple(t.shape) != tuple(shape):
-            raise InvalidArgument(7, f"{what} has shape {tuple(t.shape)}, not {tuple(shape)}")
-        return t
 
-    def _rows_tensor(self, t, what: str, dtypes, shape=None):
-        """A 2-d tensor whose rows are contiguous, with the stride from one row to the next."""
-        self._tensor(t, what, dtypes, shape)
-        if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+    def _rows_tensor(self, t, what: str, dtypes):
+        """Address, rows, columns and row stride of a 2-d tensor whose rows are contiguous."""
+        self._check_tensor(t, what, dtypes)
+        if t.dim() != 2:
             raise InvalidArgument(7, f"{what} must be a 2-d tensor with contiguous rows")
-        return t, int(t.stride(0)) if t.shape[0] > 1 else int(t.shape[1])
+        (rows, cols), (ld, step) = t.shape, t.stride()
+        if cols > 1 and step != 1:
+            raise InvalidArgument(7, f"{what} must be a 2-d tensor with contiguous rows")
+        return t.data_ptr(), rows, cols, ld if rows > 1 else cols
 
-    def _row_vector(self, t, what: str, dtype, rows: int, cols: int | None = None):
-        self._tensor(t, what, (dtype,), (rows,) if cols is None else (rows, cols))
+    def _row_vector(self, t, what: str, dtype, shape) -> int:
+        self._check_tensor(t, what, (dtype,))
+        if t.shape != shape:
+            raise InvalidArgument(7, f"{what} has shape {tuple(t.shape)}, not {shape}")
         if not t.is_contiguous():
             raise InvalidArgument(7, f"{what} must be contiguous")
-        return t
+        return t.data_ptr()
 
     def _out(self, out, name: str, dtype, shape):
-        torch = _torch()
-        t = (out or {}).get(name)
+        t = out.get(name) if out else None
         if t is None:
-            return torch.empty(shape, dtype=dtype, device=f"cuda:{self.device}")
-        self._tensor(t, name, (dtype,), shape)
-        if not t.is_contiguous():
-            raise InvalidArgument(7, f"{name} must be contiguous")
+            return _torch().empty(shape, dtype=dtype, device=self._dev)
+        self._row_vector(t, name, dtype, shape)
         return t
 
     def _logits(self, logits) -> Logits:
-        torch = _torch()
-        codes = {torch.float32: "f32", torch.float16: "f16", torch.bfloat16: "bf16"}
-        t, ld = self._rows_tensor(logits, "logits", tuple(codes))
-        return Logits(_ptr(t), int(t.shape[0]), int(t.shape[1]), ld, DTYPES[codes[t.dtype]], 0)
+        codes = _logit_codes()
+        ptr, rows, vocab, ld = self._rows_tensor(logits, "logits", codes)
+        return Logits(ptr, rows, vocab, ld, codes[logits.dtype], 0)
 
     def _token_mask(self, mask, x: Logits):
         torch = _torch()
-        if mask is None:
-            return None, 0
         words = (x.vocab + 63) // 64
+        self._check_tensor(mask, "mask", (torch.int64,))
         if mask.dim() == 1:
-            self._tensor(mask, "mask", (torch.int64,), (words,))
-            if words > 1 and mask.stride(0) != 1:
-                raise InvalidArgument(7, "mask must be contiguous")
-            return mask, 0
-        t, ld = self._rows_tensor(mask, "mask", (torch.int64,), (x.rows, words))
-        return t, ld
+            return self._row_vector(mask, "mask", torch.int64, (words,)), 0
+        ptr, rows, cols, ld = self._rows_tensor(mask, "mask", (torch.int64,))
+        if rows != x.rows or cols != words:
+            raise InvalidArgument(7, f"mask has shape {tuple(mask.shape)}, not {(x.rows, words)}")
+        return ptr, ld
 
     def top_logits(self, logits, k: int, temperature: float = 1.0, mask=None, lse: bool = True,
                    out: dict | None = None, stream=None, sync: bool = True) -> dict:
@@ -394,38 +412,45 @@ class Context:
         (tbgb_top_logits).  NaN, -inf and masked logits are never taken; short rows end in (-inf, -1)."""
         torch = _torch()
         x = self._logits(logits)
-        m, mld = self._token_mask(mask, x)
-        if not 1 <= int(k) <= 1024:
+        m, mld = self._token_mask(mask, x) if mask is not None else (None, 0)
+        k = int(k)
+        if not 1 <= k <= 1024:
             raise InvalidArgument(7, "k must be in [1, 1024]")
-        handle, scope = self._stream_scope(stream, logits, m, *(out or {}).values())
-        with scope:
-            res = {"values": self._out(out, "values", logits.dtype, (x.rows, int(k))),
-                   "ids": self._out(out, "ids", torch.int32, (x.rows, int(k)))}
-            if lse:
-                res["lse"] = self._out(out, "lse", torch.float32, (x.rows,))
-        self._check(self._L.tbgb_top_logits(self._h, C.byref(x), int(k), float(temperature), _ptr(m), mld,
-                                            _ptr(res["values"]), _ptr(res["ids"]), _ptr(res.get("lse")), handle))
+
+        def outputs():
+            return (self._out(out, "values", logits.dtype, (x.rows, k)), self._out(out, "ids", torch.int32, (x.rows, k)),
+                    self._out(out, "lse", torch.float32, (x.rows,)) if lse else None)
+
+        if stream is None:
+            handle = _current_stream(self.device)
+            v, i, e = outputs()
+        else:
+            handle, scope = self._scope(stream, logits, mask, *(out or {}).values())
+            with scope:
+                v, i, e = outputs()
+        self._check(self._L.tbgb_top_logits(self._h, x, k, temperature, m, mld, v.data_ptr(), i.data_ptr(),
+                                            e.data_ptr() if lse else None, handle))
         if sync:
             self.sync(handle)
-        return res
+        return {"values": v, "ids": i, "lse": e} if lse else {"values": v, "ids": i}
 
     def _teacher(self, x: Logits, ids, teacher, teacher_lse, temperature) -> Teacher:
         torch = _torch()
-        codes = {torch.float32: "f32", torch.float16: "f16", torch.bfloat16: "bf16"}
-        ids, ids_ld = self._rows_tensor(ids, "ids", (torch.int32,))
-        t, ld = self._rows_tensor(teacher, "teacher", tuple(codes), (x.rows, int(ids.shape[1])))
-        if int(ids.shape[0]) != x.rows:
-            raise InvalidArgument(7, "ids and logits must have the same number of rows")
-        if teacher_lse is not None:
-            self._row_vector(teacher_lse, "teacher_lse", torch.float32, x.rows)
-        return Teacher(_ptr(ids), _ptr(t), _ptr(teacher_lse), ids_ld, ld, DTYPES[codes[t.dtype]], int(ids.shape[1]),
-                       float(temperature), 0)
+        codes = _logit_codes()
+        ids_ptr, rows, k, ids_ld = self._rows_tensor(ids, "ids", (torch.int32,))
+        ptr, t_rows, t_k, ld = self._rows_tensor(teacher, "teacher", codes)
+        if rows != x.rows or t_rows != rows or t_k != k:
+            raise InvalidArgument(7, "logits, ids and teacher must have the same number of rows, ids and teacher of columns")
+        lse = self._row_vector(teacher_lse, "teacher_lse", torch.float32, (rows,)) if teacher_lse is not None else None
+        return Teacher(ids_ptr, ptr, lse, ids_ld, ld, codes[teacher.dtype], k, temperature, 0)
 
     def _gradient(self, grad, logits):
-        torch = _torch()
         if grad is None:
-            grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        return self._rows_tensor(grad, "grad", (logits.dtype,), logits.shape)
+            grad = _torch().empty(logits.shape, dtype=logits.dtype, device=self._dev)
+        ptr, rows, cols, ld = self._rows_tensor(grad, "grad", (logits.dtype,))
+        if grad.shape != logits.shape:
+            raise InvalidArgument(7, "grad and logits must have the same shape")
+        return grad, ptr, ld
 
     def distill_loss(self, logits, ids, teacher, teacher_lse=None, temperature: float = 1.0,
                      out: dict | None = None, stream=None, sync: bool = True) -> dict:
@@ -436,15 +461,21 @@ class Context:
         torch = _torch()
         x = self._logits(logits)
         t = self._teacher(x, ids, teacher, teacher_lse, temperature)
-        handle, scope = self._stream_scope(stream, logits, ids, teacher, teacher_lse, *(out or {}).values())
-        with scope:
-            res = {"loss": self._out(out, "loss", torch.float32, (x.rows,)),
-                   "stats": self._out(out, "stats", torch.float32, (x.rows, 2))}
-        self._check(self._L.tbgb_distill_loss(self._h, C.byref(x), C.byref(t), _ptr(res["loss"]), _ptr(res["stats"]),
-                                              handle))
+
+        def outputs():
+            return (self._out(out, "loss", torch.float32, (x.rows,)), self._out(out, "stats", torch.float32, (x.rows, 2)))
+
+        if stream is None:
+            handle = _current_stream(self.device)
+            loss, stats = outputs()
+        else:
+            handle, scope = self._scope(stream, logits, ids, teacher, teacher_lse, *(out or {}).values())
+            with scope:
+                loss, stats = outputs()
+        self._check(self._L.tbgb_distill_loss(self._h, x, t, loss.data_ptr(), stats.data_ptr(), handle))
         if sync:
             self.sync(handle)
-        return res
+        return {"loss": loss, "stats": stats}
 
     def distill_grad(self, logits, ids, teacher, stats, weight, teacher_lse=None, temperature: float = 1.0, grad=None,
                      stream=None, sync: bool = True):
@@ -453,13 +484,16 @@ class Context:
         torch = _torch()
         x = self._logits(logits)
         t = self._teacher(x, ids, teacher, teacher_lse, temperature)
-        self._row_vector(stats, "stats", torch.float32, x.rows, 2)
-        self._row_vector(weight, "weight", torch.float32, x.rows)
-        handle, scope = self._stream_scope(stream, logits, ids, teacher, teacher_lse, stats, weight, grad)
-        with scope:
-            g, ld = self._gradient(grad, logits)
-        self._check(self._L.tbgb_distill_grad(self._h, C.byref(x), C.byref(t), _ptr(stats), _ptr(weight), _ptr(g), ld,
-                                              handle))
+        st = self._row_vector(stats, "stats", torch.float32, (x.rows, 2))
+        w = self._row_vector(weight, "weight", torch.float32, (x.rows,))
+        if stream is None:
+            handle = _current_stream(self.device)
+            g, ptr, ld = self._gradient(grad, logits)
+        else:
+            handle, scope = self._scope(stream, logits, ids, teacher, teacher_lse, stats, weight, grad)
+            with scope:
+                g, ptr, ld = self._gradient(grad, logits)
+        self._check(self._L.tbgb_distill_grad(self._h, x, t, st, w, ptr, ld, handle))
         if sync:
             self.sync(handle)
         return g
@@ -471,18 +505,23 @@ class Context:
         torch = _torch()
         x = self._logits(logits)
         t = self._teacher(x, ids, teacher, teacher_lse, temperature)
-        self._row_vector(weight, "weight", torch.float32, x.rows)
-        handle, scope = self._stream_scope(stream, logits, ids, teacher, teacher_lse, weight, grad,
-                                           *(out or {}).values())
-        with scope:
-            g, ld = self._gradient(grad, logits)
-            res = {"loss": self._out(out, "loss", torch.float32, (x.rows,)),
-                   "stats": self._out(out, "stats", torch.float32, (x.rows, 2)), "grad": g}
-        self._check(self._L.tbgb_distill_step(self._h, C.byref(x), C.byref(t), _ptr(weight), _ptr(res["loss"]),
-                                              _ptr(res["stats"]), _ptr(g), ld, handle))
+        w = self._row_vector(weight, "weight", torch.float32, (x.rows,))
+
+        def outputs():
+            return (*self._gradient(grad, logits), self._out(out, "loss", torch.float32, (x.rows,)),
+                    self._out(out, "stats", torch.float32, (x.rows, 2)))
+
+        if stream is None:
+            handle = _current_stream(self.device)
+            g, ptr, ld, loss, stats = outputs()
+        else:
+            handle, scope = self._scope(stream, logits, ids, teacher, teacher_lse, weight, grad, *(out or {}).values())
+            with scope:
+                g, ptr, ld, loss, stats = outputs()
+        self._check(self._L.tbgb_distill_step(self._h, x, t, w, loss.data_ptr(), stats.data_ptr(), ptr, ld, handle))
         if sync:
             self.sync(handle)
-        return res
+        return {"loss": loss, "stats": stats, "grad": g}
 
     def sample_tokens(self, logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, mask=None, logprobs: bool = True,
                       out: dict | None = None, stream=None, sync: bool = True) -> dict:
@@ -492,27 +531,44 @@ class Context:
         top_p >= 1 and min_p <= 0 are off.  A row without any token to take gets -1 and -inf."""
         torch = _torch()
         x = self._logits(logits)
-        self._row_vector(u, "u", torch.float32, x.rows)
-        m, mld = self._token_mask(mask, x)
+        rows = (x.rows,)
+        up = self._row_vector(u, "u", torch.float32, rows)
+        m, mld = self._token_mask(mask, x) if mask is not None else (None, 0)
         p = Sampling()
-        kept = []
-        for name, value, dtype in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
-                                   ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
-            if isinstance(value, torch.Tensor):
-                kept.append(self._row_vector(value, name, dtype, x.rows))
-                setattr(p, name, _ptr(value))
-            else:
-                setattr(p, name + "_all", int(value) if name == "top_k" else float(value))
-        handle, scope = self._stream_scope(stream, logits, u, m, *kept, *(out or {}).values())
-        with scope:
-            res = {"tokens": self._out(out, "tokens", torch.int32, (x.rows,))}
-            if logprobs:
-                res["logprobs"] = self._out(out, "logprobs", torch.float32, (x.rows,))
-        self._check(self._L.tbgb_sample_tokens(self._h, C.byref(x), _ptr(u), C.byref(p), _ptr(m), mld,
-                                               _ptr(res["tokens"]), _ptr(res.get("logprobs")), handle))
+        if isinstance(temperature, torch.Tensor):
+            p.temperature = self._row_vector(temperature, "temperature", torch.float32, rows)
+        else:
+            p.temperature_all = temperature
+        if isinstance(top_k, torch.Tensor):
+            p.top_k = self._row_vector(top_k, "top_k", torch.int32, rows)
+        else:
+            p.top_k_all = int(top_k)
+        if isinstance(top_p, torch.Tensor):
+            p.top_p = self._row_vector(top_p, "top_p", torch.float32, rows)
+        else:
+            p.top_p_all = top_p
+        if isinstance(min_p, torch.Tensor):
+            p.min_p = self._row_vector(min_p, "min_p", torch.float32, rows)
+        else:
+            p.min_p_all = min_p
+
+        def outputs():
+            return (self._out(out, "tokens", torch.int32, rows),
+                    self._out(out, "logprobs", torch.float32, rows) if logprobs else None)
+
+        if stream is None:
+            handle = _current_stream(self.device)
+            tokens, lp = outputs()
+        else:
+            settings = [v for v in (temperature, top_k, top_p, min_p) if isinstance(v, torch.Tensor)]
+            handle, scope = self._scope(stream, logits, u, mask, *settings, *(out or {}).values())
+            with scope:
+                tokens, lp = outputs()
+        self._check(self._L.tbgb_sample_tokens(self._h, x, up, p, m, mld, tokens.data_ptr(),
+                                               lp.data_ptr() if logprobs else None, handle))
         if sync:
             self.sync(handle)
-        return res
+        return {"tokens": tokens, "logprobs": lp} if logprobs else {"tokens": tokens}
 
     def groupby_hash_into(self, keys, a, max_groups: int, out_keys, out: dict, n_groups, b=None, c=None,
                           expr: str = "a", pred: str | None = None, threshold: float = 0.0, mask=None,
