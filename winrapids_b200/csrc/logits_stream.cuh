@@ -227,6 +227,26 @@ __device__ __forceinline__ void collect_top(const Stream<T, NT, MASK>& st, int K
   if (tid == 0 && sm.n_el > li.el_cap) sm.spilled = 1;
 }
 
+// list[0, n) without what lies below a bound of the K-th largest; the new n (all of it where that is not more than
+// sort_list takes quickly).
+template <int NT>
+__device__ __forceinline__ int prune_list(BoundSmem& sm, unsigned long long* list, unsigned long long* spare, int* count,
+                                          int n, int K) {
+  if (n <= 256 || K > 224) return n;
+  const int tid = threadIdx.x;
+  if (tid == 0) *count = 0;
+  const float tau = kth_bound<NT>(sm, K, [&](auto g) {
+    for (int i = tid; i < n; i += NT) g(Elem<float>::unkey(static_cast<uint32_t>(list[i] >> 32)));
+  });
+  for (int i = tid; i < n; i += NT)
+    if (Elem<float>::unkey(static_cast<uint32_t>(list[i] >> 32)) >= tau) spare[atomicAdd(count, 1)] = list[i];
+  __syncthreads();
+  n = *count;
+  for (int i = tid; i < n; i += NT) list[i] = spare[i];
+  __syncthreads();
+  return n;
+}
+
 // Sorts list[0, n), largest first, n <= cap (a power of two).
 template <int NT>
 __device__ __forceinline__ void sort_list(unsigned long long* list, int n) {

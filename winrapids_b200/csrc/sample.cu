@@ -29,7 +29,7 @@ constexpr float kGrid = 1073741824.0f;  // 2^30
 
 struct Weight {
   float zmax, scale;
-  __device__ __forceinline__ float power(float z) const { return z == zmax ? 1.0f : exp2f((z - zmax) * scale); }
+  __device__ __forceinline__ float power(float z) const { return z == zmax ? 1.0f : power2((z - zmax) * scale); }
   // 0 for -inf (and for the NaN of -inf at an infinite temperature)
   __device__ __forceinline__ unsigned unit(float z) const { return __float2uint_rn(power(z) * kGrid); }
   __device__ __forceinline__ unsigned long long operator()(float z) const { return unit(z); }
@@ -293,16 +293,19 @@ __device__ __noinline__ void exact_row(const SampleArgs& a, long long r, ExactSm
 // instruction on the special function units, which are busy for most of the pass with the power itself.
 
 constexpr int kParts = 1024;       // of the exponent's range
+constexpr int kPartBytes = 9 * 1024;  // two counters for each, later the search's arrays
 // Tokens of the part that holds the end of the prefix: equal 16-bit logits between 16 and 32 are up to one in 30 of a
 // vocabulary with a spread of 2.
 constexpr int kEdgeMost = 4096;
 constexpr float kSmall = 0.0078125f;  // 2^-7
 
+static_assert(2 * 4 * (kParts + 2) <= kPartBytes, "counters");
+
 struct SampleSmem {
   TopSmem top;
   float f[32];
   unsigned long long w[32];
-  unsigned long long cta_w, above, cut;
+  unsigned long long cta_w, above;
   float cta_f;
   int n_edge, part;
   unsigned long long sub[32];
@@ -465,6 +468,105 @@ struct Sampler {
   }
 };
 
+struct CutSmem {
+  unsigned long long mass[512], few[256], most, least, rem;
+  unsigned count[512];
+  int bin, n;
+};
+
+static_assert(sizeof(CutSmem) <= kPartBytes, "the search takes the place of the counters");
+
+// The entry of list[0, n) (in no order) at which the running sum of weight(entry), from the largest entry down, reaches
+// `need`; the sum of the list reaches it.  The range of entries that holds it is cut into 512 equal parts
+// until no more than 256 entries are left: by their keys first, by their ids where keys are equal.
+template <int NT, typename W>
+__device__ __forceinline__ unsigned long long cut_of(CutSmem& sm, const unsigned long long* list, int n,
+                                                     unsigned long long need, W weight) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tid == 0) {
+    sm.most = 0;
+    sm.least = ~0ull;
+    sm.n = 0;
+  }
+  __syncthreads();
+  unsigned long long hi = 0, lo = ~0ull;
+  for (int i = tid; i < n; i += NT) {
+    hi = max(hi, list[i]);
+    lo = min(lo, list[i]);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    hi = max(hi, __shfl_xor_sync(FULL, hi, o));
+    lo = min(lo, __shfl_xor_sync(FULL, lo, o));
+  }
+  if (lane == 0) {
+    atomicMax(&sm.most, hi);
+    atomicMin(&sm.least, lo);
+  }
+  __syncthreads();
+  hi = sm.most;
+  lo = sm.least;
+  int left = n;
+  while (left > 256) {
+    const int shift = max(55 - __clzll(static_cast<long long>(hi - lo)), 0);  // (hi - lo) >> shift < 512
+    for (int b = tid; b < 512; b += NT) {
+      sm.mass[b] = 0;
+      sm.count[b] = 0;
+    }
+    __syncthreads();
+    for (int i = tid; i < n; i += NT) {
+      const unsigned long long u = list[i];
+      if (u <= hi && u >= lo) {
+        const int b = static_cast<int>((hi - u) >> shift);
+        atomicAdd(&sm.mass[b], static_cast<unsigned long long>(weight(u)));
+        atomicAdd(&sm.count[b], 1u);
+      }
+    }
+    __syncthreads();
+    if (warp == 0) {
+      unsigned long long part = 0;
+      for (int j = 0; j < 16; ++j) part += sm.mass[lane * 16 + j];
+      const unsigned long long upto = warp_inclusive(part);
+      const int at = __ffs(__ballot_sync(FULL, upto >= need)) - 1;
+      if (lane == at) {
+        unsigned long long run = upto - part;
+        int b = lane * 16;
+        while (run + sm.mass[b] < need) run += sm.mass[b++];
+        sm.bin = b;
+        sm.rem = need - run;
+      }
+    }
+    __syncthreads();
+    const unsigned long long b = static_cast<unsigned long long>(sm.bin);
+    const unsigned long long top = hi - (b << shift), width = (1ull << shift) - 1;
+    lo = top - lo < width ? lo : top - width;
+    hi = top;
+    need = sm.rem;
+    left = static_cast<int>(sm.count[sm.bin]);
+    __syncthreads();
+  }
+  for (int i = tid; i < n; i += NT)
+    if (list[i] <= hi && list[i] >= lo) sm.few[atomicAdd(&sm.n, 1)] = list[i];
+  __syncthreads();
+  sort_list<NT>(sm.few, left);
+  if (warp == 0) {
+    unsigned long long run = 0;
+    for (int j0 = 0; j0 < left; j0 += 32) {
+      const int j = j0 + lane;
+      const unsigned long long w = j < left ? weight(sm.few[j]) : 0;
+      const unsigned long long inc = run + warp_inclusive(w);
+      const unsigned hit = __ballot_sync(FULL, j < left && inc >= need);
+      if (hit) {
+        if (lane == 0) sm.most = sm.few[j0 + __ffs(hit) - 1];
+        break;
+      }
+      run = __shfl_sync(FULL, inc, 31);
+    }
+  }
+  __syncthreads();
+  return sm.most;
+}
+
 template <typename T, int NT, bool MASK>
 __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs a, int list_k) {
   constexpr int NW = NT / 32;
@@ -520,6 +622,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
     if (C > 1) cl.sync();  // the lists have been read
     if (rank != 0) return;
     __syncthreads();
+    n = prune_list<NT>(sm.top.bound, li.el, li.vec, &sm.top.n_vec, n, k);
     sort_list<NT>(li.el, n);
     n = min(n, k);
     if (n == 0 || greedy) {
@@ -648,32 +751,30 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
   const float light = static_cast<float>(static_cast<double>(W - need) / a.x.vocab) * (1.0f / kGrid);
   const float depth = fminf(31.5f, light > 1e-12f ? 0.01f - log2f(light) : 31.5f);
   const float part_scale = kParts / depth;
-  auto part_of = [&](float z) {  // of a token: kParts and more lie below
+  auto part_of = [&](float z) {  // of a token; kParts: below them all
     const float d = z == m ? 0.0f : (z - m) * scale;
-    return static_cast<int>(fminf(-d * part_scale, 2.0f * kParts));
+    return min(static_cast<int>(-d * part_scale), kParts);
   };
   unsigned* lo = reinterpret_cast<unsigned*>(dyn);
-  unsigned* hi = lo + kParts;
-  unsigned long long* list = reinterpret_cast<unsigned long long*>(hi + kParts);
-  for (int i = tid; i < 2 * kParts; i += NT) lo[i] = 0;
+  unsigned* hi = lo + kParts + 2;
+  unsigned long long* list = reinterpret_cast<unsigned long long*>(dyn + kPartBytes);
+  for (int i = tid; i < 2 * (kParts + 2); i += NT) lo[i] = 0;
   if (tid == 0) sm.n_edge = 0;
   __syncthreads();
   float low = m - (depth / scale) * 1.00001f - fabsf(m) * 1e-6f;  // nothing below has a part
   st.each(st.a, st.b, [&](const uint4 (&x)[STEP], int) {
-#pragma unroll 1
+#pragma unroll
     for (int i = 0; i < STEP; ++i) {
-      const uint4 y = i == 0 ? x[0] : i == 1 ? x[1] : i == 2 ? x[2] : x[3];
-      if (!(Elem<T>::vmax(y) >= low)) continue;
+      if (!(Elem<T>::vmax(x[i]) >= low)) continue;
 #pragma unroll
       for (int e = 0; e < Elem<T>::EPV; ++e) {
-        const float z = Elem<T>::get(y, e);
+        const float z = Elem<T>::get(x[i], e);
         if (z >= low) {
-          const int b = part_of(z);
-          if (b < kParts) {
-            const unsigned w = sp.weight.unit(z);
-            atomicAdd(&lo[b], w & 32767u);  // 2^15 times 131072 tokens fit 32 bits
-            if (w >> 15) atomicAdd(&hi[b], w >> 15);
-          }
+          const float d = z == m ? 0.0f : (z - m) * scale;
+          const int b = min(static_cast<int>(-d * part_scale), kParts);  // (one more part for what lies below)
+          const unsigned w = __float2uint_rn(power2(d) * kGrid);
+          atomicAdd(&lo[b], w & 32767u);  // 2^15 times 131072 tokens fit 32 bits
+          if (w >> 15) atomicAdd(&hi[b], w >> 15);
         }
       }
     }
@@ -714,23 +815,22 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
   // what lies above that part, per warp, and the part's own tokens
   float edge = m - ((part + 1) / part_scale / scale) * 1.00001f - fabsf(m) * 1e-6f;
   unsigned long long mine = 0;
+  const float sure = m - ((part / part_scale) / scale) * 0.99999f + fabsf(m) * 1e-6f;  // above it no test is needed
   st.each(st.a, st.b, [&](const uint4 (&x)[STEP], int base) {
-#pragma unroll 1
+#pragma unroll
     for (int i = 0; i < STEP; ++i) {
-      const uint4 y = i == 0 ? x[0] : i == 1 ? x[1] : i == 2 ? x[2] : x[3];
-      if (!(Elem<T>::vmax(y) >= edge)) continue;
+      if (!(Elem<T>::vmax(x[i]) >= edge)) continue;
 #pragma unroll
       for (int e = 0; e < Elem<T>::EPV; ++e) {
-        const float z = Elem<T>::get(y, e);
-        if (z >= edge) {
-          const int b = part_of(z);
-          if (b < part) {
-            const float p = sp.weight.power(z);
-            if (p >= min_p) mine += __float2uint_rn(p * kGrid);
-          } else if (b == part) {
-            const int at = atomicAdd(&sm.n_edge, 1);
-            if (at < kEdgeMost) list[at] = sp.order_key(z, st.index(base + 32 * i + lane, e));
-          }
+        const float z = Elem<T>::get(x[i], e);
+        if (z < edge) continue;
+        const int b = z > sure ? -1 : part_of(z);
+        if (b < part) {
+          const float p = sp.weight.power(z);
+          if (p >= min_p) mine += __float2uint_rn(p * kGrid);
+        } else if (b == part) {
+          const int at = atomicAdd(&sm.n_edge, 1);
+          if (at < kEdgeMost) list[at] = sp.order_key(z, st.index(base + 32 * i + lane, e));
         }
       }
     }
@@ -755,25 +855,9 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
   }
   if (C > 1) cl.sync();
   else __syncthreads();
-  sort_list<NT>(all, n);
-  if (warp == 0) {
-    unsigned long long run = above;
-    unsigned long long cut = 0;
-    for (int j0 = 0; j0 < n; j0 += 32) {
-      const int j = j0 + lane;
-      const unsigned long long w = j < n ? sp.weight.unit(Elem<float>::unkey(static_cast<uint32_t>(all[j] >> 32))) : 0;
-      const unsigned long long inc = run + warp_inclusive(w);
-      const unsigned hit = __ballot_sync(FULL, j < n && inc >= need);
-      if (hit) {
-        cut = all[j0 + __ffs(hit) - 1];
-        break;
-      }
-      run = __shfl_sync(FULL, inc, 31);
-    }
-    if (lane == 0) sm.cut = cut;
-  }
-  __syncthreads();
-  const unsigned long long cut = sm.cut;
+  const unsigned long long cut = cut_of<NT>(*reinterpret_cast<CutSmem*>(lo), all, n, need - above, [&](unsigned long long u) {
+    return sp.weight.unit(Elem<float>::unkey(static_cast<uint32_t>(u >> 32)));
+  });
   auto keep = [&](float z, float p, int id) {
     if (!(p >= min_p)) return false;
     const int b = part_of(z);
@@ -801,18 +885,18 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
 
 template <typename T>
 cudaError_t launch(const SampleArgs& a, int num_sms, cudaStream_t s) {
-  constexpr int NT = 256;
+  constexpr int NT = 512;
   const long long nvec = static_cast<long long>(a.x.vocab) * sizeof(T) / 16 + 2;
   // the lists of the k largest: for the k of all rows where it is one, for 256 where rows have their own
   const int k = a.p.top_k ? 256 : a.p.top_k_all;
   const int list_k = k < 1 ? 1 : k > kTopMax ? kTopMax : k;
   // more CTAs for a row while rows leave SMs without work, a lane keeps a step and the lists hold them all
   int c = 1;
-  while (c < 8 && a.x.rows * c * 2 <= 2 * num_sms && nvec / (c * 2) >= NT && c * 2 * list_k * 5 / 4 + 64 < top_el_cap(list_k))
-    c *= 2;
+  auto more = [&] { return c < 8 && nvec / (c * 2) >= NT && c * 2 * list_k * 5 / 4 + 64 < top_el_cap(list_k); };
+  while (more() && a.x.rows * c * 2 <= 2 * num_sms) c *= 2;
   size_t smem = (static_cast<size_t>(top_vec_cap(list_k)) + top_el_cap(list_k)) * 8;
   smem = std::max(smem, sizeof(ExactSmem));
-  smem = std::max(smem, static_cast<size_t>(kParts) * 8 + (c > 1 ? 2 : 1) * kEdgeMost * 8);
+  smem = std::max(smem, static_cast<size_t>(kPartBytes) + (c > 1 ? 2 : 1) * kEdgeMost * 8);
   auto kernel = a.mask ? sample_kernel<T, NT, true> : sample_kernel<T, NT, false>;
   if (smem > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));

@@ -262,6 +262,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) top_logits_kernel(const TopArgs
   if (C > 1) cl.sync();  // the lists have been read
   if (rank != 0) return;
   __syncthreads();
+  n = prune_list<NT>(sm.bound, li.el, li.vec, &sm.n_vec, n, a.k);
   sort_list<NT>(li.el, n);
   for (int j = tid; j < a.k; j += NT) {
     const bool have = j < n;
