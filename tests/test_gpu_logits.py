@@ -651,3 +651,17 @@ def test_refusals(ctx):
         with pytest.raises(wb.InvalidArgument):
             f()
     ctx.sync()
+
+
+def test_example_runs(ctx):
+    """examples/distill_and_sample.py: the loss falls, the answers come from the record, every row is counted."""
+    import importlib.util
+    from pathlib import Path
+
+    path = Path(__file__).resolve().parents[1] / "examples" / "distill_and_sample.py"
+    spec = importlib.util.spec_from_file_location("distill_and_sample", path)
+    m = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(m)
+    got = m.main(["--rows", "256", "--vocab", "1000", "--k", "16", "--steps", "20"])
+    assert got["after"] < 0.7 * got["before"]
+    assert got["agree"] > 0.5 and got["count"] == 256
