@@ -4,7 +4,7 @@
 //                 is clear are never taken, and a row with fewer ends in (-inf, -1)
 //   lse           log sum exp(z / T) over the logits that are neither NaN nor masked
 //
-// 173 us for the 64 largest of 2048 x 131072 bf16 (3.1 TB/s), 41 us for 20 of 509 x 50001 f32 (2.5 TB/s): bound by
+// 166 us for the 64 largest of 2048 x 131072 bf16 (3.2 TB/s), 41 us for 20 of 509 x 50001 f32 (2.5 TB/s): bound by
 // instructions (11.7 an element, 5 of them the softmax) and the fixed work per row, which four CTAs of 256
 // threads an SM hide better than two of 512 (210 us).
 #include <climits>
