@@ -84,7 +84,9 @@ def _logits(case, g):
     prior = -0.7 * torch.log1p(torch.randperm(V, generator=g, device="cuda").float())
     z = torch.randn(R, V, generator=g, device="cuda").mul_(2.0).add_(prior)
     at = torch.randint(0, V, (R, 6), generator=g, device="cuda")
-    z.scatter_(1, at, 3.0 + 5.0 * torch.rand(R, 6, generator=g, device="cuda"))
+    high = 3.0 + 5.0 * torch.rand(R, 6, generator=g, device="cuda")
+    for j in range(6):  # one at a time: where a row draws a position twice, the later value stays, in every process
+        z.scatter_(1, at[:, j:j + 1], high[:, j:j + 1])
     return z
 
 
