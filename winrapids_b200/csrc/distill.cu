@@ -596,6 +596,7 @@ __global__ void __launch_bounds__(NT) distill_wide_kernel(const DistillArgs a) {
     }
     return;
   }
+  cl.sync();  // every CTA of the cluster runs: their shared memory is written below
 
   // the entries; bit (vector - v0) * EPV + e marks an element of S in this CTA's slice
   Entries en;
