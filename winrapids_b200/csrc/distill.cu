@@ -123,7 +123,8 @@ __device__ __forceinline__ RowSum row_sum(const RowPart* parts, int C, float sca
 
 constexpr long long kWaitCycles = 4000000000ll;  // about 2 s
 
-// A bounded wait (KERR_TIMEOUT when it gives up) that also acquires what other CTAs of the cluster wrote.
+// A bounded wait of a whole warp (KERR_TIMEOUT when it gives up) that also acquires what other CTAs of the
+// cluster wrote.  The answer is the same in every lane.
 __device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, uint32_t* err) {
   const uint32_t at = smem_u32(bar);
   const long long t0 = clock64();  // (the global timer takes long to read)
@@ -136,12 +137,27 @@ __device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, uint3
         : "=r"(ok)
         : "r"(at), "r"(parity)
         : "memory");
-    if (ok) return true;
-    if ((it & 255u) == 0 && clock64() - t0 > kWaitCycles) {
-      atomicOr(err, KERR_TIMEOUT);
+    if (__all_sync(FULL, ok != 0)) return true;
+    if ((it & 255u) == 0 && __any_sync(FULL, clock64() - t0 > kWaitCycles)) {
+      if ((threadIdx.x & 31) == 0) atomicOr(err, KERR_TIMEOUT);
       return false;
     }
   }
+}
+
+// The softmax warps' barrier; true when one of them brings `failed`.
+template <int NT>
+__device__ __forceinline__ bool any_failed(bool failed) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "bar.red.or.pred q, 1, %2, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(static_cast<uint32_t>(failed)), "n"(NT)
+      : "memory");
+  return r != 0;
 }
 
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
@@ -256,10 +272,7 @@ __global__ void __launch_bounds__(kRingThreads, KR > 4 ? 1 : 3) distill_kernel(c
     }
     // no copy may be in flight when the CTA ends
     for (int k = max(n - 2, 0); k < n; ++k) wait_phase(&full[k & 1], (k >> 1) & 1, a.err);
-    return;
-  }
-
-  if (warp == NW + 1) {  // the entries
+  } else if (warp == NW + 1) {  // the entries
     struct Entry {
       int id;   // -1: none, or not in this CTA's slice
       float z;  // the student's logit
@@ -419,109 +432,111 @@ __global__ void __launch_bounds__(kRingThreads, KR > 4 ? 1 : 3) distill_kernel(c
       w = next_w;
     }
     if (last_r >= 0 && r >= rows) finish();
-    return;
-  }
-
-  // the softmax and the gradient
-  const float2 scale2 = make_float2(scale, scale);
-  for (; r < rows; r += stride) {
-    const float next_w = weight_of(r + stride);
-    const RowSlice<T> sl(a, r, rank, log2c);
-    const GradRow<T> out(GRAD ? static_cast<T*>(a.grad) + r * a.grad_ld : nullptr, sl.z);
-    if (w == 0.0f) {
-      for (int j = tid; j < sl.nv; j += NT) out.store(sl.rv, sl.v0 + j, make_uint4(0, 0, 0, 0));
-      w = next_w;
-      continue;
-    }
-    const int s = n & 1, phase = (n >> 1) & 1, nv = sl.nv;
-    const uint4* stage = reinterpret_cast<const uint4*>(ring + s * cap);
-    if (!wait_phase(&full[s], phase, a.err) || !wait_phase(&ready[s], phase, a.err)) return;
-
-    // four vectors at a time; the sum is scaled when they raise the maximum
-    float m = neg_inff();
-    float2 sum = make_float2(0.0f, 0.0f);
-    auto take = [&](const uint4 (&x)[4]) {
-      float top = m;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) top = fmaxf(top, Elem<T>::vmax(x[i]));
-      if (top > m) {
-        const float f = m == neg_inff() ? 1.0f : power2((m - top) * scale);
-        sum = mul2(sum, make_float2(f, f));
-        m = top;
+  } else {  // the softmax and the gradient
+    const float2 scale2 = make_float2(scale, scale);
+    bool ok = true;  // false once a wait of this warp gave up: it then only meets the others at their barrier
+    for (; r < rows; r += stride) {
+      const float next_w = weight_of(r + stride);
+      const RowSlice<T> sl(a, r, rank, log2c);
+      const GradRow<T> out(GRAD ? static_cast<T*>(a.grad) + r * a.grad_ld : nullptr, sl.z);
+      if (w == 0.0f) {
+        for (int j = tid; j < sl.nv; j += NT) out.store(sl.rv, sl.v0 + j, make_uint4(0, 0, 0, 0));
+        w = next_w;
+        continue;
       }
-      const float ref = m == neg_inff() ? 0.0f : m;
-      const float2 minus_ref = make_float2(-ref, -ref);
+      const int s = n & 1, phase = (n >> 1) & 1, nv = sl.nv;
+      const uint4* stage = reinterpret_cast<const uint4*>(ring + s * cap);
+      ok = ok && wait_phase(&full[s], phase, a.err) && wait_phase(&ready[s], phase, a.err);
+
+      // four vectors at a time; the sum is scaled when they raise the maximum
+      float m = neg_inff();
+      float2 sum = make_float2(0.0f, 0.0f);
+      auto take = [&](const uint4 (&x)[4]) {
+        float top = m;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < Elem<T>::PAIRS; ++j) sum = add2(sum, power2(Elem<T>::pair(x[i], j), minus_ref, scale2));
-    };
-    int v = tid;
-    for (; v + 3 * NT < nv; v += 4 * NT) {
-      const uint4 x[4] = {stage[v], stage[v + NT], stage[v + 2 * NT], stage[v + 3 * NT]};
-      take(x);
-    }
-    if (v < nv) {
-      uint4 x[4] = {stage[v], RowView<T>::none(), RowView<T>::none(), RowView<T>::none()};
-#pragma unroll
-      for (int i = 1; i < 4; ++i)
-        if (v + i * NT < nv) x[i] = stage[v + i * NT];
-      take(x);
-    }
-    __syncwarp();
-    if (!GRAD && lane == 0) mbar_arrive(&done[s]);
-    const float m_w = warp_max(m);
-    const float s_w = warp_sum(scaled(m, sum.x + sum.y, m_w, scale));
-    if (lane == 0) w_ms[warp] = make_float2(m_w, s_w);
-    asm volatile("bar.sync 1, %0;" ::"n"(NT) : "memory");
-    if (warp == 0) {
-      const float2 ms = lane < NW ? w_ms[lane] : make_float2(neg_inff(), 0.0f);
-      if (!wait_phase(&counted[s], phase, a.err)) return;
-      RowPart part = entries_part[s];
-      part.m = ms.x;
-#pragma unroll
-      for (int o = NW > 8 ? 8 : 4; o > 0; o >>= 1) part.m = fmaxf(part.m, __shfl_xor_sync(FULL, part.m, o));
-      part.s = scaled(ms.x, ms.y, part.m, scale);
-#pragma unroll
-      for (int o = NW > 8 ? 8 : 4; o > 0; o >>= 1) part.s += __shfl_xor_sync(FULL, part.s, o);
-      if (lane < C) send_part(&parts[n & 3][rank], &heard[s], lane, part);
-    }
-    if (!wait_phase(&heard[s], phase, a.err)) return;
-    if (GRAD) {
-      const RowSum t = row_sum(parts[n & 3], C, scale);
-      const float inv = __fdividef(1.0f, t.total);
-      float f = w * inv_t * inv;
-      if (with_tail && t.p < 1.0f && t.s_out > 0.0f)
-        f = w * inv_t * __fdividef(t.p - t.s_in * inv, t.s_out);  // (p(S) - q(S)) / q_r / total
-      const float2 minus_ref = make_float2(-t.ref, -t.ref), f2 = make_float2(f, f);
-      auto give = [&](const uint4& x) {
-        uint4 g;
-#pragma unroll
-        for (int j = 0; j < Elem<T>::PAIRS; ++j)
-          Elem<T>::set_pair(g, j, mul2(power2(Elem<T>::pair(x, j), minus_ref, scale2), f2));
-        return g;
-      };
-      if (out.same) {
-        // whole vectors at once, the row's partial ends by elements
-        uint4* to = reinterpret_cast<uint4*>(out.base) + sl.v0;
-        int v = tid + sl.w0;
-        for (; v + 3 * NT < sl.w1; v += 4 * NT) {
-          const uint4 x[4] = {stage[v], stage[v + NT], stage[v + 2 * NT], stage[v + 3 * NT]};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) __stcs(to + v + i * NT, give(x[i]));
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, Elem<T>::vmax(x[i]));
+        if (top > m) {
+          const float f = m == neg_inff() ? 1.0f : power2((m - top) * scale);
+          sum = mul2(sum, make_float2(f, f));
+          m = top;
         }
-        for (; v < sl.w1; v += NT) __stcs(to + v, give(stage[v]));
-        if (tid == 0 && sl.w0 > 0) out.store(sl.rv, sl.v0, give(stage[0]));
-        if (tid == NT - 1 && sl.w1 < nv && sl.w1 >= sl.w0) out.store(sl.rv, sl.v0 + nv - 1, give(stage[nv - 1]));
-      } else {
-        for (int v = tid; v < nv; v += NT) out.store(sl.rv, sl.v0 + v, give(stage[v]));
+        const float ref = m == neg_inff() ? 0.0f : m;
+        const float2 minus_ref = make_float2(-ref, -ref);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < Elem<T>::PAIRS; ++j) sum = add2(sum, power2(Elem<T>::pair(x[i], j), minus_ref, scale2));
+      };
+      int v = ok ? tid : nv;
+      for (; v + 3 * NT < nv; v += 4 * NT) {
+        const uint4 x[4] = {stage[v], stage[v + NT], stage[v + 2 * NT], stage[v + 3 * NT]};
+        take(x);
+      }
+      if (v < nv) {
+        uint4 x[4] = {stage[v], RowView<T>::none(), RowView<T>::none(), RowView<T>::none()};
+#pragma unroll
+        for (int i = 1; i < 4; ++i)
+          if (v + i * NT < nv) x[i] = stage[v + i * NT];
+        take(x);
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&done[s]);
+      if (!GRAD && ok && lane == 0) mbar_arrive(&done[s]);
+      const float m_w = warp_max(m);
+      const float s_w = warp_sum(scaled(m, sum.x + sum.y, m_w, scale));
+      if (lane == 0) w_ms[warp] = make_float2(m_w, s_w);
+      if (any_failed<NT>(!ok)) break;  // every one of these warps, or none
+      if (warp == 0) {
+        const float2 ms = lane < NW ? w_ms[lane] : make_float2(neg_inff(), 0.0f);
+        ok = wait_phase(&counted[s], phase, a.err);
+        RowPart part = entries_part[s];
+        part.m = ms.x;
+#pragma unroll
+        for (int o = NW > 8 ? 8 : 4; o > 0; o >>= 1) part.m = fmaxf(part.m, __shfl_xor_sync(FULL, part.m, o));
+        part.s = scaled(ms.x, ms.y, part.m, scale);
+#pragma unroll
+        for (int o = NW > 8 ? 8 : 4; o > 0; o >>= 1) part.s += __shfl_xor_sync(FULL, part.s, o);
+        if (ok && lane < C) send_part(&parts[n & 3][rank], &heard[s], lane, part);
+      }
+      ok = ok && wait_phase(&heard[s], phase, a.err);
+      if (GRAD && ok) {
+        const RowSum t = row_sum(parts[n & 3], C, scale);
+        const float inv = __fdividef(1.0f, t.total);
+        float f = w * inv_t * inv;
+        if (with_tail && t.p < 1.0f && t.s_out > 0.0f)
+          f = w * inv_t * __fdividef(t.p - t.s_in * inv, t.s_out);  // (p(S) - q(S)) / q_r / total
+        const float2 minus_ref = make_float2(-t.ref, -t.ref), f2 = make_float2(f, f);
+        auto give = [&](const uint4& x) {
+          uint4 g;
+#pragma unroll
+          for (int j = 0; j < Elem<T>::PAIRS; ++j)
+            Elem<T>::set_pair(g, j, mul2(power2(Elem<T>::pair(x, j), minus_ref, scale2), f2));
+          return g;
+        };
+        if (out.same) {
+          // whole vectors at once, the row's partial ends by elements
+          uint4* to = reinterpret_cast<uint4*>(out.base) + sl.v0;
+          int v = tid + sl.w0;
+          for (; v + 3 * NT < sl.w1; v += 4 * NT) {
+            const uint4 x[4] = {stage[v], stage[v + NT], stage[v + 2 * NT], stage[v + 3 * NT]};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) __stcs(to + v + i * NT, give(x[i]));
+          }
+          for (; v < sl.w1; v += NT) __stcs(to + v, give(stage[v]));
+          if (tid == 0 && sl.w0 > 0) out.store(sl.rv, sl.v0, give(stage[0]));
+          if (tid == NT - 1 && sl.w1 < nv && sl.w1 >= sl.w0) out.store(sl.rv, sl.v0 + nv - 1, give(stage[nv - 1]));
+        } else {
+          for (int v = tid; v < nv; v += NT) out.store(sl.rv, sl.v0 + v, give(stage[v]));
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&done[s]);
+      }
+      ++n;
+      w = next_w;
     }
-    ++n;
-    w = next_w;
   }
+  // peers may still send to this CTA, also after one of its waits gave up
+  __syncwarp();
+  cl.sync();
 }
 
 // The row's entries in shared memory: id (-1: none, also an id outside the vocabulary, which is
