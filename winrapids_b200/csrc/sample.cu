@@ -295,7 +295,7 @@ __device__ __noinline__ void exact_row(const SampleArgs& a, long long r, ExactSm
 // over 256 x 131072 bf16; 512 threads a row (256: 197 and 34 us, 1024: 130 and 47).
 
 constexpr int kParts = 1024;       // of the exponent's range
-constexpr int kPartBytes = 9 * 1024;  // two counters for each, later the search's arrays
+constexpr int kPartBytes = 9 * 1024;  // two words for each, later the search's arrays
 // Tokens of the part that holds the end of the prefix: equal 16-bit logits between 16 and 32 are up to one in 30 of a
 // vocabulary with a spread of 2.
 constexpr int kEdgeMost = 4096;
@@ -718,10 +718,9 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
     return;
   }
   const float scale = 1.4426950408889634f / temperature;
-  // NaN, infinite logits, an infinite temperature, many more than the lists hold: the exact row
+  // NaN, infinite logits, an infinite temperature, a k past the lists: the exact row
   const bool cut_p = top_p < 1.0f;
-  if (!(m <= 3.402823466e38f) || !(scale > 0.0f) || (top_k > 0 && top_k < a.x.vocab) ||
-      (cut_p && a.x.vocab / C > 131072)) {
+  if (!(m <= 3.402823466e38f) || !(scale > 0.0f) || (top_k > 0 && top_k < a.x.vocab)) {
     exact();
     return;
   }
@@ -775,8 +774,9 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
           const float d = z == m ? 0.0f : (z - m) * scale;
           const int b = min(static_cast<int>(-d * part_scale), kParts);  // (one more part for what lies below)
           const unsigned w = __float2uint_rn(power2(d) * kGrid);
-          atomicAdd(&lo[b], w & 32767u);  // 2^15 times 131072 tokens fit 32 bits
-          if (w >> 15) atomicAdd(&hi[b], w >> 15);
+          // a part's sum in two words, the carry taken from the low one's old value: exact for any number of tokens
+          // (a u32 pair of 15 + 16 bits wraps at 131072 tokens of weight 1)
+          if (atomicAdd(&lo[b], w) > ~w) atomicAdd(&hi[b], 1u);
         }
       }
     }
@@ -787,7 +787,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
   for (int b = tid; b < kParts; b += NT) {
     unsigned long long v = 0;
     for (int c = 0; c < C; ++c)
-      v += cl.map_shared_rank(lo, c)[b] + (static_cast<unsigned long long>(cl.map_shared_rank(hi, c)[b]) << 15);
+      v += cl.map_shared_rank(lo, c)[b] + (static_cast<unsigned long long>(cl.map_shared_rank(hi, c)[b]) << 32);
     list[b] = v;
   }
   __syncthreads();
