@@ -382,8 +382,11 @@ typedef struct {
 /* KL divergence of the student q = softmax(z / temperature) from the teacher, per row (in nats):
  *   loss[r]  = sum p_i (log p_i - log q_i)  [+ p_r (log p_r - log q_r), the other-token outcome;
  *              left out where the student has no logit above -inf outside the entries]
- *   stats[r] = (log sum exp(z / temperature), factor): what tbgb_distill_grad needs again
- * A row without entries has loss 0.  NaN or +inf logits, and a row of nothing but -inf, make the
+ *   stats[r] = (log sum exp(z / temperature), factor): what tbgb_distill_grad needs again; factor is
+ *              that of q_j in the gradient outside the entries, 1 where there is no other-token outcome
+ * The gradient by z_j, times temperature: q_j - p_j at an entry, factor q_j elsewhere; without the
+ * other-token outcome P q_j - p_j and P q_j, P the sum of the entries' p (1 for a closed teacher).
+ * A row without entries has loss and gradient 0.  NaN or +inf logits, and a row of nothing but -inf, make the
  * row's loss and gradient NaN.  An id outside [-1, vocab) makes tbgb_sync report
  * TBGB_ERR_KEY_OUT_OF_RANGE (the entry is left out), an id named twice in a row
  * TBGB_ERR_INVALID_ARGUMENT (the row's outputs are then unspecified). */

@@ -56,11 +56,13 @@ def distill(z, ids, t, lse, temperature, weight=1.0):
     x = z / temperature
     L = logsumexp(x)
     logq = x - L
-    logp = t - (logsumexp(t) if lse is None else float(lse))
+    norm = logsumexp(t) if lse is None else float(lse)
+    logp = t - norm if lse is not None or norm > -np.inf else np.full(len(t), -np.inf)
     p = np.exp(logp)
     with np.errstate(invalid="ignore"):
         terms = np.where(p > 0, p * (logp - logq[ids]), 0.0)
     loss, mag, off = terms.sum(), np.abs(terms).sum(), 1.0
+    whole = p.sum()  # the loss is a sum over the entries alone: its p are a part (or nothing) of a distribution
     if lse is not None:
         p_r = 1.0 - p.sum()
         out = np.ones(len(z), bool)
@@ -69,9 +71,9 @@ def distill(z, ids, t, lse, temperature, weight=1.0):
         if p_r > 0 and q_r > 0:
             loss += p_r * (np.log(p_r) - np.log(q_r))
             mag += abs(p_r * np.log(p_r)) + abs(p_r * np.log(q_r))
-            off = 1.0 - p_r / q_r
-    g = np.exp(logq) * off
-    g[ids] = np.exp(logq[ids]) - p
+            off, whole = 1.0 - p_r / q_r, None
+    g = np.exp(logq) * (off if whole is None else whole)
+    g[ids] = np.exp(logq[ids]) * (1.0 if whole is None else whole) - p
     return loss, (L, off), g * weight / temperature, mag
 
 

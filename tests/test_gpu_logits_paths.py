@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 import logits_ref as ref
-from test_gpu_logits import DT, check_sample, host, table, tdt
+from test_gpu_logits import DT, EPS, TINY, check_sample, host, record, table, tdt
 
 pytestmark = pytest.mark.gpu
 
@@ -65,3 +65,78 @@ def test_top_p_of_long_rows_with_many_rows(ctx, rows, vocab, dtype):
         zr = host(z)[r % 3]
         want = zr[j] - zr.max() - np.log(W / ref.GRID)
         assert abs(lp[r] - want) <= 4e-6 * (1 + abs(want)), r
+
+
+# ---- distillation ---------------------------------------------------------------------------------
+
+
+def check_rows(ctx, z, ids, t, lse, T, dtype, weight=None, rows=None):
+    """Loss, gradient from the stats, and step.  An element's gradient w / T (P q - p) carries 4e-6 of q and p as in
+    test_gpu_logits.py and the error of P, 2^-24 times 4 units of a power and the additions of a tree: 5e-6 in all."""
+    import torch
+
+    if weight is None:
+        weight = torch.linspace(0.5, 1.5, z.shape[0], device="cuda")
+    a = ctx.distill_loss(z, ids, t, teacher_lse=lse, temperature=T)
+    g = ctx.distill_grad(z, ids, t, a["stats"], weight, teacher_lse=lse, temperature=T)
+    b = ctx.distill_step(z, ids, t, weight, teacher_lse=lse, temperature=T)
+    for r in range(z.shape[0]) if rows is None else rows:
+        zh, ih, w = host(z[r]), host(ids[r]), float(weight[r])
+        loss, _, grad, mag = ref.distill(zh, ih, host(t[r]), None if lse is None else float(lse[r]), T, w)
+        q = np.exp(zh / T - ref.logsumexp(zh / T))
+        tol = w / T * 5e-6 * q + 5e-6 * np.abs(grad) + EPS[dtype] * np.abs(grad) + TINY[dtype]
+        have = ih[ih >= 0]
+        tol[have] += 5e-6 * np.abs(w / T * q[have] - grad[have])  # of p
+        for got, what in ((g, "grad"), (b["grad"], "step")):
+            d = np.abs(host(got[r]) - grad)
+            assert (d <= tol).all(), (what, r, int(np.argmax(d - tol)), float((d - tol).max()))
+        if w != 0:
+            for got, what in ((a, "loss"), (b, "step")):
+                assert abs(float(got["loss"][r]) - loss) <= 4e-6 * mag + 1e-6, (what, r, float(got["loss"][r]), loss)
+        else:
+            assert float(b["loss"][r]) == 0.0 and (host(b["grad"][r]) == 0).all()
+    return a, g, b
+
+
+WIDE = {"f32": 240000, "f16": 470000, "bf16": 470001}  # longer than a cluster's stages
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("size", ["small", "wide"])
+@pytest.mark.parametrize("k", [9, 200])
+def test_distill_rows_whose_entries_are_no_distribution(ctx, size, dtype, k):
+    """Closed rows without an entry (or none above -inf) have neither loss nor gradient; where the outcome outside
+    the record is missing the gradient is P q - p."""
+    import torch
+
+    V = 1003 if size == "small" else WIDE[dtype]
+    T = 1.25
+    z = table(4, V, dtype, 41, spread=1.5)
+    ids, t, lse = record(z, k, T, 3, dtype, True)
+    ids[1] = -1
+    t[2] = -float("inf")
+    a, g, b = check_rows(ctx, z, ids, t, None, T, dtype)
+    for r in (1, 2):
+        assert float(a["loss"][r]) == 0.0 and (host(g[r]) == 0).all() and (host(b["grad"][r]) == 0).all()
+    # a masked vocabulary: nothing outside the entries; the recorded p sum to 0.7
+    ids, t, _ = record(z, k, T, 3, dtype, False)
+    lse = (torch.logsumexp(t.double() / T, 1) - np.log(0.7)).float()
+    out = torch.ones(4, V, dtype=torch.bool, device="cuda")
+    out.scatter_(1, ids.long(), False)
+    z = z.masked_fill(out, -float("inf"))
+    a, g, b = check_rows(ctx, z, ids, t, lse, T, dtype)
+    assert (a["stats"][:, 1] == 1).all() and (b["stats"][:, 1] == 1).all()
+    w = host(torch.linspace(0.5, 1.5, 4))
+    for got in (g, b["grad"]):
+        assert np.abs(host(got).sum(1)).max() <= (w / T * (5e-6 + 2 * EPS[dtype])).max() + V * TINY[dtype]
+
+
+@pytest.mark.parametrize("dtype", DT)
+def test_distill_whole_vocabulary_of_a_part_of_the_teacher(ctx, dtype):
+    import torch
+
+    T = 0.8
+    z = table(3, 301, dtype, 2)
+    ids, t, _ = record(z, 301, T, 2, dtype, False)
+    lse = (torch.logsumexp(t.double() / T, 1) - np.log(0.4)).float()
+    check_rows(ctx, z, ids, t, lse, T, dtype)

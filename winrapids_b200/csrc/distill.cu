@@ -10,8 +10,11 @@
 //   loss = sum p_i (log p_i - log q_i) + p_r (log p_r - log q_r)
 //   T dloss/dz_j = q_j - p_j in S,  q_j (1 - p_r / q_r) = q_j (p(S) - q(S)) / q_r outside
 // A row whose student has no weight outside S, and one whose teacher has none there, have no such
-// outcome.  stats[r] = (log sum exp(z / T), the factor of q_j outside S) is what the backward pass
-// needs of the forward pass.
+// outcome: their loss is the sum over S alone, whose p sum to P = p(S), and
+//   T dloss/dz_j = P q_j - p_j in S,  P q_j outside
+// (P = 1 for a closed teacher with an entry, 0 without one).  stats[r] = (log sum exp(z / T), the factor of
+// q_j outside S, 1 where the outcome is missing) is what the backward pass needs of the forward pass; P it
+// takes from the record.
 #include <algorithm>
 #include <climits>
 
@@ -231,6 +234,9 @@ __global__ void __launch_bounds__(kRingThreads, KR > 4 ? 1 : 3) distill_kernel(c
   cl.sync();
 
   auto weight_of = [&](long long r) { return GRAD && r < rows ? a.weight[r] : 1.0f; };
+  auto rest_counts = [&](const RowSum& t) { return with_tail && t.p < 1.0f && t.s_out > 0.0f; };
+  // P of a row without the outcome outside S; a closed teacher's p sum to 1 but for their rounding
+  auto whole = [&](const RowSum& t) { return with_tail || t.p == 0.0f ? t.p : 1.0f; };
   int n = 0;  // rows taken so far (padding rows are not counted)
   long long r = blockIdx.x >> log2c;
   float w = weight_of(r);
@@ -336,7 +342,7 @@ __global__ void __launch_bounds__(kRingThreads, KR > 4 ? 1 : 3) distill_kernel(c
       const float inv = __fdividef(1.0f, t.total);
       if (rank == 0 && lane == 0) {
         float loss = t.loss, off = 1.0f;
-        if (with_tail && t.p < 1.0f && t.s_out > 0.0f) {
+        if (rest_counts(t)) {
           const float q_in = t.s_in * inv, q_out = t.s_out * inv;
           const float lq = q_in < 0.5f ? log1pf(-q_in) : logf(q_out);
           loss += (1.0f - t.p) * (log1pf(-t.p) - lq);
@@ -349,11 +355,11 @@ __global__ void __launch_bounds__(kRingThreads, KR > 4 ? 1 : 3) distill_kernel(c
       if (!GRAD) return true;
       if (!wait_phase(&done[s], phase, a.err)) return false;  // over what the others have stored
       T* g = static_cast<T*>(a.grad) + last_r * a.grad_ld;
-      const float wt = last_w * inv_t;
+      const float wt = last_w * inv_t, q_factor = inv * (rest_counts(t) ? 1.0f : whole(t));
 #pragma unroll
       for (int i = 0; i < KR; ++i)
         if (before[i].id >= 0)
-          store_elem<T>(g, before[i].id, wt * (power2((before[i].z - t.ref) * scale) * inv - before[i].p));
+          store_elem<T>(g, before[i].id, wt * (power2((before[i].z - t.ref) * scale) * q_factor - before[i].p));
       return true;
     };
     fetch(r);
@@ -501,9 +507,9 @@ __global__ void __launch_bounds__(kRingThreads, KR > 4 ? 1 : 3) distill_kernel(c
       if (GRAD && ok) {
         const RowSum t = row_sum(parts[n & 3], C, scale);
         const float inv = __fdividef(1.0f, t.total);
-        float f = w * inv_t * inv;
-        if (with_tail && t.p < 1.0f && t.s_out > 0.0f)
-          f = w * inv_t * __fdividef(t.p - t.s_in * inv, t.s_out);  // (p(S) - q(S)) / q_r / total
+        const float f = w * inv_t *
+                        (rest_counts(t) ? __fdividef(t.p - t.s_in * inv, t.s_out)  // (p(S) - q(S)) / q_r / total
+                                        : whole(t) * inv);
         const float2 minus_ref = make_float2(-t.ref, -t.ref), f2 = make_float2(f, f);
         auto give = [&](const uint4& x) {
           uint4 g;
@@ -547,8 +553,8 @@ struct Entries {
   float* p;
 };
 
-// Called by one warp: p of every entry and the sum of them.  log2p is left in `p` by the loader.
-__device__ __forceinline__ float entry_probs(const DistillArgs& a, const Entries& en, long long r) {
+// Called by one warp: p of every entry (the loader left the teacher's logit in its place) and, asked for, their sum.
+__device__ __forceinline__ float entry_probs(const DistillArgs& a, const Entries& en, long long r, bool with_sum) {
   const int lane = threadIdx.x & 31;
   float sum = 0.0f;
   if (a.teacher_lse) {
@@ -561,7 +567,7 @@ __device__ __forceinline__ float entry_probs(const DistillArgs& a, const Entries
       en.p[k] = t == neg_inff() ? 0.0f : power2((q - lse + rest) * kLog2e);
       sum += en.p[k];
     }
-    return warp_sum(sum);
+    return with_sum ? warp_sum(sum) : 0.0f;
   }
   float m = neg_inff();
   for (int k = lane; k < a.k; k += 32)
@@ -639,7 +645,7 @@ __global__ void __launch_bounds__(NT) distill_wide_kernel(const DistillArgs a) {
   }
   __syncthreads();
   if (warp == 0) {
-    const float s = entry_probs(a, en, r);
+    const float s = entry_probs(a, en, r, true);
     if (lane == 0) p_sum = s;
   }
 
@@ -734,6 +740,7 @@ __global__ void __launch_bounds__(NT) distill_wide_kernel(const DistillArgs a) {
 template <typename T, int NT>
 __global__ void __launch_bounds__(NT, 1024 / NT) distill_grad_kernel(const DistillArgs a, int tiles) {
   extern __shared__ uint32_t smem[];
+  __shared__ float p_sum, stat[2];
   const long long r = blockIdx.x / tiles;
   const int rank = static_cast<int>(blockIdx.x - r * tiles);
   const int tid = threadIdx.x;
@@ -746,12 +753,14 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_grad_kernel(const Disti
     for (int v = sl.v0 + tid; v < sl.v1; v += NT) out.store(sl.rv, v, make_uint4(0, 0, 0, 0));
     return;
   }
+  if (tid >= NT - 2) stat[tid - (NT - 2)] = a.stats[2 * r + tid - (NT - 2)];  // (the first threads have entries to fetch)
   sl.load(0);
   Entries en;
   en.id = reinterpret_cast<int*>(smem);
   en.z = reinterpret_cast<float*>(smem) + a.k;
   en.p = en.z + a.k;
   const int lo = max(sl.rv.first(sl.v0), 0), hi = min(sl.rv.first(sl.v1), a.x.vocab);
+  int some = 0;  // an entry above -inf
   for (int k = tid; k < a.k; k += NT) {
     int id = a.ids[r * a.ids_ld + k];
     if (id < -1 || id >= a.x.vocab) {
@@ -760,11 +769,25 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_grad_kernel(const Disti
     }
     en.id[k] = id;
     en.p[k] = id >= 0 ? teacher_logit(a, r * a.teacher_ld + k) : 0.0f;
+    some |= id >= 0 && !(en.p[k] == neg_inff());
     if (id >= lo && id < hi) en.z[k] = Elem<T>::from_bits(Elem<T>::load_bits(z_row + id));
   }
-  __syncthreads();
-  if (tid < 32) entry_probs(a, en, r);
-  const float inv_t = 1.0f / a.temperature, lse = a.stats[2 * r], off = a.stats[2 * r + 1];
+  if (a.teacher_lse)
+    __syncthreads();
+  else
+    some = __syncthreads_or(some);
+  const float inv_t = 1.0f / a.temperature, lse = stat[0];
+  float off = stat[1];
+  const bool missing = off == 1.0f;  // the outcome outside S (where it is there, P is 1 but for its rounding)
+  const float P = tid < 32 ? entry_probs(a, en, r, missing) : 0.0f;
+  if (missing) {  // the same for the whole CTA; a closed teacher's P is known without the sum
+    off = some ? 1.0f : 0.0f;
+    if (a.teacher_lse) {
+      if (tid == 0) p_sum = P;
+      __syncthreads();
+      off = p_sum;
+    }
+  }
   const float wt = w * inv_t;
   auto q = [&](float z) { return power2((z * inv_t - lse) * kLog2e); };
   const float2 inv2 = make_float2(inv_t, inv_t), minus_lse = make_float2(-lse, -lse),
@@ -784,7 +807,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_grad_kernel(const Disti
   }
   __syncthreads();
   for (int k = tid; k < a.k; k += NT)
-    if (en.id[k] >= lo && en.id[k] < hi) store_elem<T>(g_row, en.id[k], wt * (q(en.z[k]) - en.p[k]));
+    if (en.id[k] >= lo && en.id[k] < hi) store_elem<T>(g_row, en.id[k], wt * ((missing ? off : 1.0f) * q(en.z[k]) - en.p[k]));
 }
 
 template <typename K>
