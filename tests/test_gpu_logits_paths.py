@@ -140,3 +140,63 @@ def test_distill_whole_vocabulary_of_a_part_of_the_teacher(ctx, dtype):
     ids, t, _ = record(z, 301, T, 2, dtype, False)
     lse = (torch.logsumexp(t.double() / T, 1) - np.log(0.4)).float()
     check_rows(ctx, z, ids, t, lse, T, dtype)
+
+
+def far_outside(dtype, V, T, gap, spread=1.0):
+    """Rows whose logits outside the record lie `gap` (in units of T) below those in it, with a teacher that leaves 0.2
+    outside."""
+    import torch
+
+    z = table(3, V, dtype, 51, spread=spread)
+    ids, t, _ = record(z, 12, T, 3, dtype, False)
+    lse = (torch.logsumexp(t.double() / T, 1) - np.log(0.8)).float()
+    out = torch.ones_like(z, dtype=torch.bool)
+    out.scatter_(1, ids.long(), False)
+    z = torch.where(out, (z.float() - gap * T).to(z.dtype), z)
+    return z, ids, t, lse, out
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("T,gap", [(1.0, 70.0), (0.1, 75.0), (1.0, 120.0), (0.1, 120.0), (2.0, 3000.0), (1.0, 40000.0)])
+@pytest.mark.parametrize("size", ["small", "wide"])
+def test_distill_other_tokens_far_below_the_entries(ctx, dtype, T, gap, size):
+    """The other-token outcome counts however small the student's probability of it is: the loss has p_r log q_r.
+    z / T of the outside logits is a rounded number of the size of the gap: 2^-23 of it in the exponent's argument."""
+    import torch
+
+    V = 1003 if size == "small" else WIDE[dtype]
+    z, ids, t, lse, out = far_outside(dtype, V, T, gap)
+    w = torch.tensor([1.0, 0.5, 2.0], device="cuda")
+    a = ctx.distill_loss(z, ids, t, teacher_lse=lse, temperature=T)
+    b = ctx.distill_step(z, ids, t, w, teacher_lse=lse, temperature=T)
+    g = ctx.distill_grad(z, ids, t, a["stats"], w, teacher_lse=lse, temperature=T)
+    for r in range(3):
+        zh, ih = host(z[r]), host(ids[r])
+        # (the restatement's q_r underflows too at a gap of thousands: the loss by its logarithm); the temperature is the
+        # 32-bit number that the call takes
+        x = zh / float(np.float32(T))
+        L, o = ref.logsumexp(x), host(out[r])
+        logp = host(t[r]) / float(np.float32(T)) - float(lse[r])
+        p, lq_r = np.exp(logp), ref.logsumexp(x[o]) - L
+        p_r = 1.0 - p.sum()
+        terms = np.append(p * (logp - x[ih] + L), p_r * (np.log(p_r) - lq_r))
+        loss, mag = terms.sum(), np.abs(terms).sum()
+        wr = float(w[r])
+        q = np.exp(x - L)
+        # q_j / q_r (p(S) - q(S)), with powers of two below 2^-126 of the largest there 0
+        e = np.where(o & ((x - x[o].max()) / np.log(2.0) >= -126), np.exp(np.where(o, x, -np.inf) - ref.logsumexp(x[o])), 0.0)
+        grad = e * (p.sum() - q[ih].sum()) * wr / T
+        grad[ih] = (q[ih] - p) * wr / T
+        tol = 1e-5 * np.abs(grad) + EPS[dtype] * np.abs(grad) + TINY[dtype] + 1e-38
+        tol[ih] += 5e-6 * wr / T * (q[ih] + p)
+        for got in (a, b):
+            assert abs(float(got["loss"][r]) - loss) <= 4e-6 * mag + 1e-6, (r, float(got["loss"][r]), loss)
+        d = np.abs(host(b["grad"][r]) - grad)
+        assert (d <= tol).all(), (r, int(np.argmax(d - tol)), float(d.max()))
+        if lq_r > -86:  # the factor of q_j and its stats are within the type's range
+            # (there it is the product q_j factor whose power of two is 0 below 2^-126)
+            rel = 2e-5 + 3 * 2.0 ** -23 * abs(lq_r)
+            want = np.where(o & (np.abs(grad) < 2.0 ** -126 * wr / T), 0.0, grad)
+            d = np.abs(host(g[r]) - want)
+            assert (d <= tol + rel * np.abs(want)).all(), (r, float(d.max()))
+        assert np.isfinite(host(g[r])).all()

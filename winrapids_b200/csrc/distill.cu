@@ -9,8 +9,9 @@
 //   loses everything when the student has learnt the entries)
 //   loss = sum p_i (log p_i - log q_i) + p_r (log p_r - log q_r)
 //   T dloss/dz_j = q_j - p_j in S,  q_j (1 - p_r / q_r) = q_j (p(S) - q(S)) / q_r outside
-// A row whose student has no weight outside S, and one whose teacher has none there, have no such
-// outcome: their loss is the sum over S alone, whose p sum to P = p(S), and
+// The sum outside S is carried by its own largest logit: however far below the entries it lies, log q_r and
+// q_j / q_r are as exact as any.  A row whose student has no logit above -inf outside S, and one whose teacher
+// has nothing there, have no such outcome: their loss is the sum over S alone, whose p sum to P = p(S), and
 //   T dloss/dz_j = P q_j - p_j in S,  P q_j outside
 // (P = 1 for a closed teacher with an entry, 0 without one).  stats[r] = (log sum exp(z / T), the factor of
 // q_j outside S, 1 where the outcome is missing) is what the backward pass needs of the forward pass; P it
@@ -32,6 +33,13 @@ __device__ __forceinline__ float teacher_logit(const DistillArgs& a, long long i
   if (a.teacher_dtype == TBGB_F32) return static_cast<const float*>(a.teacher)[i];
   if (a.teacher_dtype == TBGB_F16) return __half2float(static_cast<const __half*>(a.teacher)[i]);
   return __bfloat162float(static_cast<const __nv_bfloat16*>(a.teacher)[i]);
+}
+
+// log2 of p = exp(t / T - lse): the quotient's own rounding is put back, it would be the error of log p
+__device__ __forceinline__ float tail_log2(float t, float lse, float temperature, float inv_t) {
+  const float q = t * inv_t;
+  const float rest = fabsf(q) < 1e30f ? fmaf(-q, temperature, t) * inv_t : 0.0f;
+  return t == neg_inff() ? neg_inff() : (q - lse + rest) * kLog2e;
 }
 
 template <typename T>
@@ -78,8 +86,8 @@ struct GradRow {
 //   others     the running maximum and sum over the stage, the exchange of six numbers per CTA over
 //              distributed shared memory, then the gradient from the stage
 // The three overlap across rows and across the CTAs of an SM.  Bound by that chain per row (copy, entries, sums,
-// exchange, gradient) with three CTAs an SM to hide it: 484 us for 4096 x 131072 bf16 with 64 entries (4.4 TB/s of the
-// 2.15 GB that the step reads and writes), 126 us for the loss alone over 2048 x 100003 f16 (3.3 TB/s).
+// exchange, gradient) with three CTAs an SM to hide it: 486 us for 4096 x 131072 bf16 with 64 entries (4.4 TB/s of the
+// 2.15 GB that the step reads and writes), 131 us for the loss alone over 2048 x 100003 f16 (3.1 TB/s).
 
 __device__ __forceinline__ float scaled(float m, float s, float top, float scale) {
   return m == neg_inff() || m == top ? s : s * power2((m - top) * scale);
@@ -93,35 +101,71 @@ struct RowPart {  // a CTA's part of a row
 };
 
 struct RowSum {
-  float ref, total, s_in, s_out, loss, p;
+  float ref, total, s_in;  // largest logit of all (0 for none), the whole sum and S's by it
+  float m_out, s_out;      // largest logit outside S, the sum there by that
+  float loss, p;
 };
 
-// Every part's sums by the largest logit of all, the same in every lane: lane c takes CTA c's part
-// (a loop over them is a chain of latencies that stands between the two passes over a row).
+// The row's sums from its parts, the same in every lane: lane c takes CTA c's part
+// (a loop over them is a chain of latencies that stands between the two passes over a row).  LOSS: with the loss, which
+// only the warp that writes it needs.
+template <bool LOSS>
 __device__ __forceinline__ RowSum row_sum(const RowPart* parts, int C, float scale) {
   const int lane = threadIdx.x & 31;
   RowPart p{neg_inff(), 0.0f, neg_inff(), 0.0f, 0.0f, 0.0f};
   if ((lane & 7) < C) p = parts[lane & 7];
-  float m = fmaxf(p.m, p.ms);
-#pragma unroll
-  for (int o = 4; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(FULL, m, o));
   RowSum t;
+  t.m_out = p.m;
+  float m = p.ms;
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) {
+    t.m_out = fmaxf(t.m_out, __shfl_xor_sync(FULL, t.m_out, o));
+    m = fmaxf(m, __shfl_xor_sync(FULL, m, o));
+  }
+  m = fmaxf(m, t.m_out);
   t.ref = m == neg_inff() ? 0.0f : m;
-  t.s_out = scaled(p.m, p.s, m, scale);
+  t.s_out = scaled(p.m, p.s, t.m_out, scale);
   t.s_in = scaled(p.ms, p.ss, m, scale);
   t.p = p.p;
   t.loss = p.loss;
-  if (p.p > 0.0f && p.ms > neg_inff()) t.loss -= p.p * ((p.ms - t.ref) * scale * kLn2);
+  if (LOSS && p.p > 0.0f && p.ms > neg_inff()) t.loss -= p.p * ((p.ms - t.ref) * scale * kLn2);
 #pragma unroll
   for (int o = 4; o > 0; o >>= 1) {
     t.s_out += __shfl_xor_sync(FULL, t.s_out, o);
     t.s_in += __shfl_xor_sync(FULL, t.s_in, o);
     t.p += __shfl_xor_sync(FULL, t.p, o);
-    t.loss += __shfl_xor_sync(FULL, t.loss, o);
+    if (LOSS) t.loss += __shfl_xor_sync(FULL, t.loss, o);
   }
-  t.total = t.s_in + t.s_out;
-  t.loss += t.p * log2f(t.total) * kLn2;
+  t.total = t.s_in + scaled(t.m_out, t.s_out, m, scale);
+  if (LOSS) t.loss += t.p * log2f(t.total) * kLn2;
   return t;
+}
+
+// Whether "a token outside S" is one of the row's outcomes.
+__device__ __forceinline__ bool rest_counts(const RowSum& t, bool with_tail) {
+  return with_tail && t.p < 1.0f && t.m_out > neg_inff();
+}
+// P of a row without it; a closed teacher's p sum to 1 but for their rounding.
+__device__ __forceinline__ float whole(const RowSum& t, bool with_tail) { return with_tail || t.p == 0.0f ? t.p : 1.0f; }
+
+// Loss and stats, by one thread.
+__device__ __forceinline__ void write_row(const DistillArgs& a, long long r, const RowSum& t, float scale) {
+  float loss = t.loss, off = 1.0f;
+  if (rest_counts(t, a.teacher_lse != nullptr)) {
+    const float inv = __fdividef(1.0f, t.total), q_in = t.s_in * inv;
+    const float q_out = scaled(t.m_out, t.s_out, t.ref, scale) * inv;
+    // (the logarithms apart lose digits where they are near one another, and the quotient where it underflows)
+    const float lq = q_in < 0.5f      ? log1pf(-q_in)
+                     : q_out >= 1e-30f ? logf(q_out)
+                                       : (t.m_out - t.ref) * scale * kLn2 + logf(t.s_out) - logf(t.total);
+    loss += (1.0f - t.p) * (log1pf(-t.p) - lq);
+    off = __fdividef(t.p - q_in, q_out);  // (to 2 units; an exact division in this chain costs the step 1 %)
+    if (fabsf(off) > 3.402823466e38f) off = copysignf(3.402823466e38f, off);  // q_out below the type's range
+    if (t.p == q_in) off = 0.0f;
+  }
+  a.loss[r] = loss;
+  a.stats[2 * r] = t.total > 0.0f ? t.ref / a.temperature + logf(t.total) : neg_inff() + t.total;
+  a.stats[2 * r + 1] = off;
 }
 
 constexpr long long kWaitCycles = 4000000000ll;  // about 2 s
@@ -234,9 +278,6 @@ __global__ void __launch_bounds__(kRingThreads, KR > 4 ? 1 : 3) distill_kernel(c
   cl.sync();
 
   auto weight_of = [&](long long r) { return GRAD && r < rows ? a.weight[r] : 1.0f; };
-  auto rest_counts = [&](const RowSum& t) { return with_tail && t.p < 1.0f && t.s_out > 0.0f; };
-  // P of a row without the outcome outside S; a closed teacher's p sum to 1 but for their rounding
-  auto whole = [&](const RowSum& t) { return with_tail || t.p == 0.0f ? t.p : 1.0f; };
   int n = 0;  // rows taken so far (padding rows are not counted)
   long long r = blockIdx.x >> log2c;
   float w = weight_of(r);
@@ -314,12 +355,7 @@ __global__ void __launch_bounds__(kRingThreads, KR > 4 ? 1 : 3) distill_kernel(c
       }
       if (with_tail) {
 #pragma unroll
-        for (int i = 0; i < KR; ++i) {
-          // t / T - lse: the quotient's own rounding is put back, it would be the error of log p
-          const float q = t[i] * inv_t;
-          const float rest = fabsf(q) < 1e30f ? fmaf(-q, a.temperature, t[i]) * inv_t : 0.0f;
-          now[i].l = t[i] == neg_inff() ? neg_inff() : (q - ahead_lse + rest) * kLog2e;
-        }
+        for (int i = 0; i < KR; ++i) now[i].l = tail_log2(t[i], ahead_lse, a.temperature, inv_t);
       } else {
         m = warp_max(m);
         const float ref = m == neg_inff() ? 0.0f : m;
@@ -338,24 +374,13 @@ __global__ void __launch_bounds__(kRingThreads, KR > 4 ? 1 : 3) distill_kernel(c
     auto finish = [&]() {  // loss, stats and the entries' gradients of the row before
       const int s = last_n & 1, phase = (last_n >> 1) & 1;
       if (!wait_phase(&heard[s], phase, a.err)) return false;
-      const RowSum t = row_sum(parts[last_n & 3], C, scale);
-      const float inv = __fdividef(1.0f, t.total);
-      if (rank == 0 && lane == 0) {
-        float loss = t.loss, off = 1.0f;
-        if (rest_counts(t)) {
-          const float q_in = t.s_in * inv, q_out = t.s_out * inv;
-          const float lq = q_in < 0.5f ? log1pf(-q_in) : logf(q_out);
-          loss += (1.0f - t.p) * (log1pf(-t.p) - lq);
-          off = __fdividef(t.p - q_in, q_out);
-        }
-        a.loss[last_r] = loss;
-        a.stats[2 * last_r] = t.total > 0.0f ? t.ref / a.temperature + logf(t.total) : neg_inff() + t.total;
-        a.stats[2 * last_r + 1] = off;
-      }
+      const RowSum t = row_sum<true>(parts[last_n & 3], C, scale);
+      if (rank == 0 && lane == 0) write_row(a, last_r, t, scale);
       if (!GRAD) return true;
       if (!wait_phase(&done[s], phase, a.err)) return false;  // over what the others have stored
       T* g = static_cast<T*>(a.grad) + last_r * a.grad_ld;
-      const float wt = last_w * inv_t, q_factor = inv * (rest_counts(t) ? 1.0f : whole(t));
+      const float wt = last_w * inv_t;
+      const float q_factor = __fdividef(rest_counts(t, with_tail) ? 1.0f : whole(t, with_tail), t.total);
 #pragma unroll
       for (int i = 0; i < KR; ++i)
         if (before[i].id >= 0)
@@ -505,12 +530,13 @@ __global__ void __launch_bounds__(kRingThreads, KR > 4 ? 1 : 3) distill_kernel(c
       }
       ok = ok && wait_phase(&heard[s], phase, a.err);
       if (GRAD && ok) {
-        const RowSum t = row_sum(parts[n & 3], C, scale);
+        const RowSum t = row_sum<false>(parts[n & 3], C, scale);
         const float inv = __fdividef(1.0f, t.total);
-        const float f = w * inv_t *
-                        (rest_counts(t) ? __fdividef(t.p - t.s_in * inv, t.s_out)  // (p(S) - q(S)) / q_r / total
-                                        : whole(t) * inv);
-        const float2 minus_ref = make_float2(-t.ref, -t.ref), f2 = make_float2(f, f);
+        const bool rest = rest_counts(t, with_tail);
+        // outside S: 2^((z - m_out) scale) (p(S) - q(S)) / s_out, or P 2^((z - ref) scale) / total
+        const float f = w * inv_t * (rest ? __fdividef(t.p - t.s_in * inv, t.s_out) : whole(t, with_tail) * inv);
+        const float ref = rest ? t.m_out : t.ref;
+        const float2 minus_ref = make_float2(-ref, -ref), f2 = make_float2(f, f);
         auto give = [&](const uint4& x) {
           uint4 g;
 #pragma unroll
@@ -553,7 +579,8 @@ struct Entries {
   float* p;
 };
 
-// Called by one warp: p of every entry (the loader left the teacher's logit in its place) and, asked for, their sum.
+// Called by one warp: log2 p of every entry in the place of the teacher's logit (LOG), or p and, asked for, their sum.
+template <bool LOG>
 __device__ __forceinline__ float entry_probs(const DistillArgs& a, const Entries& en, long long r, bool with_sum) {
   const int lane = threadIdx.x & 31;
   float sum = 0.0f;
@@ -561,10 +588,8 @@ __device__ __forceinline__ float entry_probs(const DistillArgs& a, const Entries
     const float lse = a.teacher_lse[r], inv_t = 1.0f / a.temperature;
     for (int k = lane; k < a.k; k += 32) {
       if (en.id[k] < 0) continue;
-      // t / T - lse: the quotient's own rounding is put back, it would be the error of log p
-      const float t = en.p[k], q = t * inv_t;
-      const float rest = fabsf(q) < 1e30f ? fmaf(-q, a.temperature, t) * inv_t : 0.0f;
-      en.p[k] = t == neg_inff() ? 0.0f : power2((q - lse + rest) * kLog2e);
+      const float l = tail_log2(en.p[k], lse, a.temperature, inv_t);
+      en.p[k] = LOG ? l : power2(l);
       sum += en.p[k];
     }
     return with_sum ? warp_sum(sum) : 0.0f;
@@ -574,7 +599,7 @@ __device__ __forceinline__ float entry_probs(const DistillArgs& a, const Entries
     if (en.id[k] >= 0) m = fmaxf(m, en.p[k]);
   m = warp_max(m);
   if (m == neg_inff()) {
-    for (int k = lane; k < a.k; k += 32) en.p[k] = 0.0f;
+    for (int k = lane; k < a.k; k += 32) en.p[k] = LOG ? neg_inff() : 0.0f;
     return 0.0f;
   }
   const float scale = kLog2e / a.temperature;
@@ -583,33 +608,31 @@ __device__ __forceinline__ float entry_probs(const DistillArgs& a, const Entries
   sum = warp_sum(sum);
   const float l2 = log2f(sum);
   for (int k = lane; k < a.k; k += 32)
-    if (en.id[k] >= 0) en.p[k] = exp2f((en.p[k] - m) * scale - l2);
+    if (en.id[k] >= 0) {
+      const float l = (en.p[k] - m) * scale - l2;
+      en.p[k] = LOG ? l : exp2f(l);
+    }
   return 1.0f;
 }
 
-struct Part {  // a CTA's part of the student's softmax
-  float m;     // largest logit
-  float out;   // sum outside S of 2^((z - m) * scale)
-  float in;    // sum over S
-};
-
-// Loss and stats of rows too long for the stages above: a cluster per row, the slices read in tiles, a bit
-// per element of the slice for the entries.
-template <typename T, int NT>
+// Rows too long for the stages above: a cluster per row, the slices read in tiles, a bit per element of the
+// slice for the entries; the gradient in a second pass over the slice.
+template <typename T, int NT, bool GRAD>
 __global__ void __launch_bounds__(NT) distill_wide_kernel(const DistillArgs a) {
   constexpr int NW = NT / 32, EPV = Elem<T>::EPV;
   extern __shared__ uint32_t smem[];
   __shared__ float w_m[NW], w_s[NW];
-  __shared__ Part parts[8];
-  __shared__ float p_sum;
+  __shared__ __align__(8) RowPart parts[8];
   cg::cluster_group cl = cg::this_cluster();
   const int C = static_cast<int>(cl.num_blocks()), rank = static_cast<int>(cl.block_rank());
   const long long r = blockIdx.x / C;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const T* z_row = static_cast<const T*>(a.x.logits) + r * a.x.ld;
   Slice<T, NT, false> sl(z_row, a.x.vocab, nullptr, rank, C);
-  const float w = a.weight ? a.weight[r] : 1.0f;
+  const GradRow<T> out_row(GRAD ? static_cast<T*>(a.grad) + r * a.grad_ld : nullptr, z_row);
+  const float w = GRAD ? a.weight[r] : 1.0f;
   if (w == 0.0f) {  // a padding row: not read
+    for (int v = sl.v0 + tid; v < sl.v1; v += NT) out_row.store(sl.rv, v, make_uint4(0, 0, 0, 0));
     if (rank == 0 && tid == 0) {
       a.loss[r] = 0.0f;
       a.stats[2 * r] = 0.0f;
@@ -637,40 +660,41 @@ __global__ void __launch_bounds__(NT) distill_wide_kernel(const DistillArgs a) {
     }
     en.id[k] = id;
     en.p[k] = id >= 0 ? teacher_logit(a, r * a.teacher_ld + k) : 0.0f;
-    if (id >= 0 && (rank == 0 || (id >= lo && id < hi))) en.z[k] = Elem<T>::from_bits(Elem<T>::load_bits(z_row + id));
     if (id >= lo && id < hi) {
+      en.z[k] = Elem<T>::from_bits(Elem<T>::load_bits(z_row + id));
       const int b = id - sl.rv.first(sl.v0);
       if (atomicOr(&bits[b >> 5], 1u << (b & 31)) & (1u << (b & 31))) atomicOr(a.err, KERR_TOKEN_TWICE);
     }
   }
   __syncthreads();
-  if (warp == 0) {
-    const float s = entry_probs(a, en, r, true);
-    if (lane == 0) p_sum = s;
-  }
+  if (warp == 0) entry_probs<true>(a, en, r, false);
 
-  // this CTA's softmax
+  // this CTA's softmax outside S
   const float scale = kLog2e / a.temperature;
   float m_w = neg_inff(), s_w = 0.0f;
-  for (int t = 0; t < sl.tiles; ++t) {
+  auto fetch = [&](int t) {  // a tile, S's places -inf
     sl.load(t);
-    float m = neg_inff(), s = 0.0f;
-    sl.each([&](float z, int, int) { m = fmaxf(m, z); });
-    m = warp_max(m);
-    const float ref = m == neg_inff() ? 0.0f : m;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int v = sl.vec(t, i);
       if (i < sl.per && v < sl.v1) {
         const int b = (v - sl.v0) * EPV;
-        const uint32_t in = bits[b >> 5] >> (b & 31);
+        const uint32_t in = (bits[b >> 5] >> (b & 31)) & ((1u << EPV) - 1);
+        if (in) {
 #pragma unroll
-        for (int e = 0; e < EPV; ++e) {
-          const float x = exp2f((Elem<T>::get(sl.r[i], e) - ref) * scale);
-          s += (in >> e) & 1u ? 0.0f : x;
+          for (int e = 0; e < EPV; ++e)
+            if ((in >> e) & 1u) Elem<T>::set(sl.r[i], e, Elem<T>::NEG_INF);
         }
       }
     }
+  };
+  for (int t = 0; t < sl.tiles; ++t) {
+    fetch(t);
+    float m = neg_inff(), s = 0.0f;
+    sl.each([&](float z, int, int) { m = fmaxf(m, z); });
+    m = warp_max(m);
+    const float ref = m == neg_inff() ? 0.0f : m;
+    sl.each([&](float z, int, int) { s += exp2f((z - ref) * scale); });
     s = warp_sum(s);
     MaxSum ms{m_w, s_w};
     ms.merge(m, s, scale);
@@ -683,56 +707,57 @@ __global__ void __launch_bounds__(NT) distill_wide_kernel(const DistillArgs a) {
   }
   __syncthreads();
   if (warp == 0) {
-    MaxSum ms{lane < NW ? w_m[lane] : neg_inff(), lane < NW ? w_s[lane] : 0.0f};
+    MaxSum out{lane < NW ? w_m[lane] : neg_inff(), lane < NW ? w_s[lane] : 0.0f};
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-      const float m2 = __shfl_xor_sync(FULL, ms.m, o), s2 = __shfl_xor_sync(FULL, ms.s, o);
-      ms.merge(m2, s2, scale);
+      const float m2 = __shfl_xor_sync(FULL, out.m, o), s2 = __shfl_xor_sync(FULL, out.s, o);
+      out.merge(m2, s2, scale);
     }
-    float in = 0.0f;
-    const float ref = ms.m == neg_inff() ? 0.0f : ms.m;
+    float ms = neg_inff(), ss = 0.0f, loss = 0.0f, ps = 0.0f;
     for (int k = lane; k < a.k; k += 32)
-      if (en.id[k] >= lo && en.id[k] < hi) in += exp2f((en.z[k] - ref) * scale);
-    in = warp_sum(in);
-    if (lane < C) *cl.map_shared_rank(&parts[rank], lane) = Part{ms.m, ms.s, in};
+      if (en.id[k] >= lo && en.id[k] < hi) ms = fmaxf(ms, en.z[k]);
+    ms = warp_max(ms);
+    const float ref = ms == neg_inff() ? 0.0f : ms;
+    for (int k = lane; k < a.k; k += 32)
+      if (en.id[k] >= lo && en.id[k] < hi) {
+        const float d = (en.z[k] - ref) * scale, p = power2(en.p[k]);
+        ss += power2(d);
+        if (p != 0.0f) loss += p * ((en.p[k] - d) * kLn2);
+        ps += p;
+      }
+    ss = warp_sum(ss);
+    loss = warp_sum(loss);
+    ps = warp_sum(ps);
+    if (lane < C) *cl.map_shared_rank(&parts[rank], lane) = RowPart{out.m, out.s, ms, ss, loss, ps};
   }
   cl.sync();
-  float m = neg_inff(), s_out = 0.0f, s_in = 0.0f;
-  for (int c = 0; c < C; ++c) m = fmaxf(m, parts[c].m);
-  const float ref = m == neg_inff() ? 0.0f : m;
-  for (int c = 0; c < C; ++c) {
-    const Part p = parts[c];
-    const float f = p.m == m ? 1.0f : exp2f((p.m - ref) * scale);
-    s_out += p.m == neg_inff() ? p.out : p.out * f;  // (a NaN reaches the sums with a maximum of -inf too)
-    s_in += p.m == neg_inff() ? p.in : p.in * f;
-  }
-  const float total = s_out + s_in, ps = p_sum;
-  const bool tail = a.teacher_lse && ps < 1.0f && s_out > 0.0f;
-  const float q_out = s_out / total;
-  const float off = tail ? (ps - s_in / total) / q_out : 1.0f;
-
-  if (rank == 0 && warp == 0) {
-    const float l2 = log2f(total);
-    float loss = 0.0f;
-    for (int k = lane; k < a.k; k += 32) {
-      if (en.id[k] < 0 || en.p[k] == 0.0f) continue;
-      const float lp = a.teacher_lse ? static_cast<float>(static_cast<double>(teacher_logit(a, r * a.teacher_ld + k)) /
-                                                              a.temperature - a.teacher_lse[r])
-                                     : logf(en.p[k]);
-      loss += en.p[k] * (lp - ((en.z[k] - ref) * scale - l2) * kLn2);
-    }
-    loss = warp_sum(loss);
-    if (tail) {
-      const float q_in = s_in / total;
-      const float lq = q_in < 0.5f ? log1pf(-q_in) : logf(q_out);
-      loss += (1.0f - ps) * (log1pf(-ps) - lq);
-    }
-    if (lane == 0) {
-      a.loss[r] = loss;
-      a.stats[2 * r] = m == neg_inff() ? neg_inff() + total : m / a.temperature + l2 * kLn2;
-      a.stats[2 * r + 1] = off;
+  const RowSum sum = row_sum<true>(parts, C, scale);
+  if (rank == 0 && tid == 0) write_row(a, r, sum, scale);
+  if (!GRAD) return;
+  const bool with_tail = a.teacher_lse != nullptr, rest = rest_counts(sum, with_tail);
+  const float wt = w / a.temperature, inv = 1.0f / sum.total, P = whole(sum, with_tail);
+  const float f = wt * (rest ? (sum.p - sum.s_in * inv) / sum.s_out : P * inv);
+  const float ref = rest ? sum.m_out : sum.ref;
+  const float2 minus_ref = make_float2(-ref, -ref), scale2 = make_float2(scale, scale), f2 = make_float2(f, f);
+  for (int t = 0; t < sl.tiles; ++t) {
+    fetch(t);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int v = sl.vec(t, i);
+      if (i < sl.per && v < sl.v1) {
+        uint4 g;
+#pragma unroll
+        for (int j = 0; j < Elem<T>::PAIRS; ++j)
+          Elem<T>::set_pair(g, j, mul2(power2(Elem<T>::pair(sl.r[i], j), minus_ref, scale2), f2));
+        out_row.store(sl.rv, v, g);
+      }
     }
   }
+  __syncthreads();
+  const float q_factor = (rest ? 1.0f : P) * inv;
+  for (int k = tid; k < a.k; k += NT)
+    if (en.id[k] >= lo && en.id[k] < hi)
+      store_elem<T>(out_row.row, en.id[k], wt * (power2((en.z[k] - sum.ref) * scale) * q_factor - power2(en.p[k])));
 }
 
 // The gradient from a forward pass's stats: one CTA per tile of NT * NV vectors of a row, held in registers.  89 us
@@ -779,7 +804,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_grad_kernel(const Disti
   const float inv_t = 1.0f / a.temperature, lse = stat[0];
   float off = stat[1];
   const bool missing = off == 1.0f;  // the outcome outside S (where it is there, P is 1 but for its rounding)
-  const float P = tid < 32 ? entry_probs(a, en, r, missing) : 0.0f;
+  const float P = tid < 32 ? entry_probs<false>(a, en, r, missing) : 0.0f;
   if (missing) {  // the same for the whole CTA; a closed teacher's P is known without the sum
     off = some ? 1.0f : 0.0f;
     if (a.teacher_lse) {
@@ -790,8 +815,11 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_grad_kernel(const Disti
   }
   const float wt = w * inv_t;
   auto q = [&](float z) { return power2((z * inv_t - lse) * kLog2e); };
-  const float2 inv2 = make_float2(inv_t, inv_t), minus_lse = make_float2(-lse, -lse),
-               log2e2 = make_float2(kLog2e, kLog2e), f_off = make_float2(wt * off, wt * off);
+  // where the factor is large, q_j underflows before their product does: it is formed in the exponent
+  const bool fold = !(fabsf(off) < 1024.0f);
+  const float c = fold ? logf(fabsf(off)) - lse : -lse, f = fold ? copysignf(wt, off) : wt * off;
+  const float2 inv2 = make_float2(inv_t, inv_t), c2 = make_float2(c, c), log2e2 = make_float2(kLog2e, kLog2e),
+               f2 = make_float2(f, f);
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int v = sl.vec(0, i);
@@ -799,8 +827,8 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_grad_kernel(const Disti
       uint4 g;
 #pragma unroll
       for (int j = 0; j < Elem<T>::PAIRS; ++j) {
-        const float2 d = mul2(add2(mul2(Elem<T>::pair(sl.r[i], j), inv2), minus_lse), log2e2);
-        Elem<T>::set_pair(g, j, mul2(make_float2(power2(d.x), power2(d.y)), f_off));
+        const float2 d = mul2(add2(mul2(Elem<T>::pair(sl.r[i], j), inv2), c2), log2e2);
+        Elem<T>::set_pair(g, j, mul2(make_float2(power2(d.x), power2(d.y)), f2));
       }
       out.store(sl.rv, v, g);
     }
@@ -844,12 +872,12 @@ cudaError_t launch(const DistillArgs& a, bool with_loss, bool with_grad, int num
     }
     constexpr int NT = 512;
     const size_t wide = static_cast<size_t>(a.k) * 12 + ((nvec + c - 1) / c * Elem<T>::EPV + 31) / 32 * 4;
-    cudaError_t e = allow_smem(distill_wide_kernel<T, NT>, wide);
-    if (e == cudaSuccess) e = launch_rows(distill_wide_kernel<T, NT>, NT, c, wide, a.x.rows, s, a);
-    if (e != cudaSuccess) return e;
-    (*launches)++;
+    auto kernel = with_grad ? distill_wide_kernel<T, NT, true> : distill_wide_kernel<T, NT, false>;
+    cudaError_t e = allow_smem(kernel, wide);
+    if (e == cudaSuccess) e = launch_rows(kernel, NT, c, wide, a.x.rows, s, a);
+    if (e == cudaSuccess) (*launches)++;
+    return e;
   }
-  if (!with_grad) return cudaSuccess;
   constexpr int NT = 512;
   constexpr long long TILE = NT * NV * 16;
   const int tiles = static_cast<int>((bytes + 32 + TILE - 1) / TILE);
