@@ -376,7 +376,7 @@ typedef struct {
   int32_t dtype;       /* of logits: F32, F16 or BF16 */
   int32_t k;           /* 1 <= k <= 1024 */
   float temperature;   /* of teacher and student, > 0 */
-  int32_t reserved;
+  int32_t stats_columns; /* floats per row of a call's stats: 2 (also 0) or 6 */
 } tbgb_teacher;
 
 /* KL divergence of the student q = softmax(z / temperature) from the teacher, per row (in nats):
@@ -384,6 +384,12 @@ typedef struct {
  *              left out where the student has no logit above -inf outside the entries]
  *   stats[r] = (log sum exp(z / temperature), factor): what tbgb_distill_grad needs again; factor is
  *              that of q_j in the gradient outside the entries, 1 where there is no other-token outcome
+ *   With stats_columns 6 a row's stats go on with (z_in, c_in, z_out, c_out): the gradient by z_j, times
+ *              temperature, is c_in e_j(z_in) - p_j at an entry and c_out e_j(z_out) elsewhere, with
+ *              e_j(m) = 2^((z_j - m) log2(e) / temperature).  From two columns q_j = exp(z_j / temperature - lse),
+ *              and every q_j carries (|lse| + |z_j / temperature|) 2^-24 of itself (nothing is left of it where the
+ *              lse of logits near the type's lowest value is not finite, or where a factor is past 3e38); six
+ *              columns give the gradient of tbgb_distill_step.
  * The gradient by z_j, times temperature: q_j - p_j at an entry, factor q_j elsewhere; without the
  * other-token outcome P q_j - p_j and P q_j, P the sum of the entries' p (1 for a closed teacher).
  * A row without entries has loss and gradient 0.  NaN or +inf logits, and a row of nothing but -inf, make the

@@ -168,7 +168,7 @@ pub struct tbgb_teacher {
     pub dtype: i32,
     pub k: i32,
     pub temperature: f32,
-    pub reserved: i32,
+    pub stats_columns: i32,
 }
 
 /// Sampling parameters: per row where the array is not null, else the same for every row.

@@ -200,3 +200,107 @@ def test_distill_other_tokens_far_below_the_entries(ctx, dtype, T, gap, size):
             d = np.abs(host(g[r]) - want)
             assert (d <= tol + rel * np.abs(want)).all(), (r, float(d.max()))
         assert np.isfinite(host(g[r])).all()
+
+
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("T", [1.0, 0.0625, 4.0])
+@pytest.mark.parametrize("offset", [0.0, 1e3, -1e3, 1e4, -1e4, 3e6])
+def test_gradient_from_saved_stats_at_any_size_of_the_logits(ctx, offset, T, tail):
+    """The gradient from six stats is the step's.  An exponent e = (z - m) log2(e) / T carries three roundings, 3 * 2^-24 of
+    its size (times ln 2) in the power; with 4e-6 of q and p as elsewhere, and 0 for a power below 2^-126."""
+    import torch
+
+    V = 2003
+    z = (table(4, V, "f32", 61, spread=1.0).double() + offset).float()
+    ids, t, lse = record(z - offset, 17, T, 3, "f32", tail)
+    w = torch.tensor([1.0, 0.5, 0.0, 2.0], device="cuda")
+    a = ctx.distill_loss(z, ids, t, teacher_lse=lse, temperature=T, full_stats=True)
+    two = ctx.distill_loss(z, ids, t, teacher_lse=lse, temperature=T)
+    assert a["stats"].shape == (4, 6) and torch.equal(a["stats"][:, :2], two["stats"]) and torch.equal(a["loss"], two["loss"])
+    g = ctx.distill_grad(z, ids, t, a["stats"], w, teacher_lse=lse, temperature=T)
+    b = ctx.distill_step(z, ids, t, w, teacher_lse=lse, temperature=T)
+    for r in range(4):
+        zh, ih, wr = host(z[r]), host(ids[r]), float(w[r])
+        _, (L, off), grad, _ = ref.distill(zh, ih, host(t[r]), None if lse is None else float(lse[r]), T, wr)
+        q = np.exp(zh / T - L)
+        q_out = 1.0 - q[ih].sum()
+        tol = (wr / T * q + np.abs(grad)) * (5e-6 + 3 * 2.0 ** -24 * (zh.max() - zh) / T) + 2.0 ** -125 * wr / T
+        tol += wr / T * q * (2e-6 / q_out if tail else 0.0)
+        tol[ih] += 5e-6 * np.abs(wr / T * q[ih] - grad[ih])
+        for got, what in ((g, "grad"), (b["grad"], "step")):
+            d = np.abs(host(got[r]) - grad)
+            assert (d <= tol).all(), (what, r, int(np.argmax(d - tol)), float((d - tol).max()))
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("T", [1.0, 0.5, 2.0])
+def test_gradient_of_a_row_of_the_lowest_value(ctx, dtype, T):
+    """Masks of the type's lowest value that leave nothing: a uniform student."""
+    import torch
+
+    V = 1000
+    z = torch.full((2, V), torch.finfo(tdt(dtype)).min, device="cuda", dtype=tdt(dtype))
+    ids, t, lse = record(table(2, V, dtype, 5), 10, T, 3, dtype, False)
+    w = torch.ones(2, device="cuda")
+    a = ctx.distill_loss(z, ids, t, temperature=T, full_stats=True)
+    g = ctx.distill_grad(z, ids, t, a["stats"], w, temperature=T)
+    b = ctx.distill_step(z, ids, t, w, temperature=T)
+    for r in range(2):
+        th = host(t[r]) / T
+        want = np.full(V, 1.0 / V / T)
+        want[host(ids[r])] -= np.exp(th - ref.logsumexp(th)) / T
+        tol = 5e-6 / T * (1.0 / V + np.abs(want)) + EPS[dtype] * np.abs(want) + TINY[dtype]
+        for got in (g, b["grad"]):
+            assert (np.abs(host(got[r]) - want) <= tol).all()
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("gap", [70.0, 120.0, 3000.0])
+@pytest.mark.parametrize("size", ["small", "wide"])
+def test_gradient_from_saved_stats_far_outside(ctx, dtype, gap, size):
+    """The student's probability outside the record is past the type's range, the gradient there is not."""
+    import torch
+
+    z, ids, t, lse, out = far_outside(dtype, 1003 if size == "small" else WIDE[dtype], 1.0, gap)
+    w = torch.tensor([1.0, 0.5, 2.0], device="cuda")
+    a = ctx.distill_loss(z, ids, t, teacher_lse=lse, full_stats=True)
+    g = host(ctx.distill_grad(z, ids, t, a["stats"], w, teacher_lse=lse))
+    b = host(ctx.distill_step(z, ids, t, w, teacher_lse=lse)["grad"])
+    assert np.isfinite(g).all() and np.abs(b).max() > 0.01
+    assert (np.abs(g - b) <= 1e-6 * np.abs(b) + 2 * EPS[dtype] * np.abs(b) + TINY[dtype] + 2.0 ** -120).all()
+
+
+def test_autograd_at_large_logits(ctx):
+    """wb.distill_loss's gradient is the step's, whatever constant the rows carry."""
+    import torch
+
+    import winrapids_b200 as wb
+
+    z = table(4, 999, "f32", 2)
+    rec = wb.top_logits(table(4, 999, "f32", 1), 25)
+    w = torch.linspace(0.5, 2.0, 4, device="cuda")
+    for c in (0.0, 8192.0):
+        x = (z + c).requires_grad_(True)
+        (wb.distill_loss(x, rec) * w).sum().backward()
+        step = ctx.distill_step(x.detach(), rec.ids, rec.values, w, teacher_lse=rec.lse)["grad"]
+        scale = float(step.abs().max())
+        assert float((x.grad - step).abs().max()) <= 2e-6 * scale
+        assert float(x.grad.sum(1).abs().max()) <= 2e-5 * scale
+
+
+def test_stats_columns_are_two_or_six(ctx):
+    import torch
+
+    import winrapids_b200 as wb
+
+    z = table(2, 100, "f32", 1)
+    ids, t, lse = record(z, 3, 1.0, 1, "f32", False)
+    w = torch.ones(2, device="cuda")
+    for cols in (1, 3, 4, 5, 7):
+        with pytest.raises(wb.InvalidArgument):
+            ctx.distill_grad(z, ids, t, torch.zeros(2, cols, device="cuda"), w)
+    with pytest.raises(wb.InvalidArgument):
+        ctx.distill_loss(z, ids, t, full_stats=True, out={"stats": torch.zeros(2, 2, device="cuda")})
+    x, teacher = ctx._logits(z), ctx._teacher(ctx._logits(z), ids, t, None, 1.0, 4)
+    loss = torch.zeros(2, device="cuda")
+    assert ctx._L.tbgb_distill_loss(ctx._h, x, teacher, loss.data_ptr(), loss.data_ptr(), None) == 7

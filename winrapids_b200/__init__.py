@@ -434,7 +434,7 @@ class Context:
             self.sync(handle)
         return {"values": v, "ids": i, "lse": e} if lse else {"values": v, "ids": i}
 
-    def _teacher(self, x: Logits, ids, teacher, teacher_lse, temperature) -> Teacher:
+    def _teacher(self, x: Logits, ids, teacher, teacher_lse, temperature, stats_columns: int = 2) -> Teacher:
         torch = _torch()
         codes = _logit_codes()
         ids_ptr, rows, k, ids_ld = self._rows_tensor(ids, "ids", (torch.int32,))
@@ -442,7 +442,7 @@ class Context:
         if rows != x.rows or t_rows != rows or t_k != k:
             raise InvalidArgument(7, "logits, ids and teacher must have the same number of rows, ids and teacher of columns")
         lse = self._row_vector(teacher_lse, "teacher_lse", torch.float32, (rows,)) if teacher_lse is not None else None
-        return Teacher(ids_ptr, ptr, lse, ids_ld, ld, codes[teacher.dtype], k, temperature, 0)
+        return Teacher(ids_ptr, ptr, lse, ids_ld, ld, codes[teacher.dtype], k, temperature, stats_columns)
 
     def _gradient(self, grad, logits):
         if grad is None:
@@ -453,17 +453,21 @@ class Context:
         return grad, ptr, ld
 
     def distill_loss(self, logits, ids, teacher, teacher_lse=None, temperature: float = 1.0,
-                     out: dict | None = None, stream=None, sync: bool = True) -> dict:
+                     out: dict | None = None, stream=None, sync: bool = True, full_stats: bool = False) -> dict:
         """Per row, the KL divergence of softmax(logits / temperature) from a teacher recorded as ids
         (int32 [rows, k], -1: unused) and teacher (its logits there): loss f32 [rows] and the stats
         [rows, 2] that distill_grad takes (tbgb_distill_loss).  With teacher_lse [rows] the teacher's
-        remaining probability is one more outcome; without it the teacher is closed among its entries."""
+        remaining probability is one more outcome; without it the teacher is closed among its entries.
+        full_stats: stats [rows, 6], from which distill_grad gives distill_step's gradient; that from [rows, 2] carries
+        the rounding of a 32-bit log-sum-exp (2^-24 of its size), which matters for large logits."""
         torch = _torch()
         x = self._logits(logits)
-        t = self._teacher(x, ids, teacher, teacher_lse, temperature)
+        columns = 6 if full_stats else 2
+        t = self._teacher(x, ids, teacher, teacher_lse, temperature, columns)
 
         def outputs():
-            return (self._out(out, "loss", torch.float32, (x.rows,)), self._out(out, "stats", torch.float32, (x.rows, 2)))
+            return (self._out(out, "loss", torch.float32, (x.rows,)),
+                    self._out(out, "stats", torch.float32, (x.rows, columns)))
 
         if stream is None:
             handle = _current_stream(self.device)
@@ -480,11 +484,12 @@ class Context:
     def distill_grad(self, logits, ids, teacher, stats, weight, teacher_lse=None, temperature: float = 1.0, grad=None,
                      stream=None, sync: bool = True):
         """The gradient of sum(weight * loss) by the logits, from the stats of distill_loss on the same
-        arguments (tbgb_distill_grad); weight f32 [rows].  `grad` may be `logits` itself."""
+        arguments (tbgb_distill_grad), of either width; weight f32 [rows].  `grad` may be `logits` itself."""
         torch = _torch()
         x = self._logits(logits)
-        t = self._teacher(x, ids, teacher, teacher_lse, temperature)
-        st = self._row_vector(stats, "stats", torch.float32, (x.rows, 2))
+        columns = 6 if isinstance(stats, torch.Tensor) and stats.shape == (x.rows, 6) else 2
+        t = self._teacher(x, ids, teacher, teacher_lse, temperature, columns)
+        st = self._row_vector(stats, "stats", torch.float32, (x.rows, columns))
         w = self._row_vector(weight, "weight", torch.float32, (x.rows,))
         if stream is None:
             handle = _current_stream(self.device)

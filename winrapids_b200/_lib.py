@@ -86,7 +86,7 @@ class Teacher(C.Structure):
 
     _fields_ = [("ids", C.c_void_p), ("logits", C.c_void_p), ("lse", C.c_void_p), ("ids_stride", C.c_int64),
                 ("logits_stride", C.c_int64), ("dtype", C.c_int32), ("k", C.c_int32), ("temperature", C.c_float),
-                ("reserved", C.c_int32)]
+                ("stats_columns", C.c_int32)]
 
 
 class Sampling(C.Structure):

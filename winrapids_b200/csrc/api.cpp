@@ -938,6 +938,8 @@ tbgb_status check_teacher(tbgb_ctx* ctx, const tbgb_logits* x, const tbgb_teache
     return fail(ctx, TBGB_ERR_INVALID_ARGUMENT, "the record's strides must be >= 0");
   if (bad_temperature(t->temperature))
     return fail(ctx, TBGB_ERR_INVALID_ARGUMENT, "temperature must be positive and finite");
+  if (t->stats_columns != 0 && t->stats_columns != 2 && t->stats_columns != 6)
+    return fail(ctx, TBGB_ERR_INVALID_ARGUMENT, "stats_columns must be 2 (or 0) or 6");
   if (misaligned(t->lse, 4)) return fail(ctx, TBGB_ERR_INVALID_ARGUMENT, "teacher lse is not 4-byte aligned");
   st = check_row_array(ctx, t->ids, x->rows, "teacher ids");
   if (st != TBGB_OK) return st;
@@ -952,6 +954,7 @@ tbgb_status check_teacher(tbgb_ctx* ctx, const tbgb_logits* x, const tbgb_teache
   a->k = t->k;
   a->teacher_lse = t->lse;
   a->temperature = t->temperature;
+  a->stats_ld = t->stats_columns == 6 ? 6 : 2;
   a->err = ctx->err;
   return TBGB_OK;
 }

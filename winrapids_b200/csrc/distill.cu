@@ -15,7 +15,9 @@
 //   T dloss/dz_j = P q_j - p_j in S,  P q_j outside
 // (P = 1 for a closed teacher with an entry, 0 without one).  stats[r] = (log sum exp(z / T), the factor of
 // q_j outside S, 1 where the outcome is missing) is what the backward pass needs of the forward pass; P it
-// takes from the record.
+// takes from the record.  A log-sum-exp in 32 bits carries 2^-24 of its size into every q_j.  Stats of six add
+// (z_in, c_in, z_out, c_out), which do not:
+//   T dloss/dz_j = c_in 2^((z - z_in) log2(e) / T) - p_j in S,  c_out 2^((z - z_out) log2(e) / T) outside
 #include <algorithm>
 #include <climits>
 
@@ -164,8 +166,23 @@ __device__ __forceinline__ void write_row(const DistillArgs& a, long long r, con
     if (t.p == q_in) off = 0.0f;
   }
   a.loss[r] = loss;
-  a.stats[2 * r] = t.total > 0.0f ? t.ref / a.temperature + logf(t.total) : neg_inff() + t.total;
-  a.stats[2 * r + 1] = off;
+  float* stats = a.stats + r * a.stats_ld;
+  stats[0] = t.total > 0.0f ? t.ref / a.temperature + logf(t.total) : neg_inff() + t.total;
+  stats[1] = off;
+  if (a.stats_ld == 6) {
+    const bool with_tail = a.teacher_lse != nullptr, rest = rest_counts(t, with_tail);
+    const float inv = __fdividef(1.0f, t.total), P = whole(t, with_tail);
+    stats[2] = t.ref;
+    stats[3] = rest ? inv : P * inv;
+    stats[4] = rest ? t.m_out : t.ref;
+    stats[5] = rest ? __fdividef(t.p - t.s_in * inv, t.s_out) : P * inv;
+  }
+}
+
+// The same of a padding row.
+__device__ __forceinline__ void write_padding(const DistillArgs& a, long long r) {
+  a.loss[r] = 0.0f;
+  for (int i = 0; i < a.stats_ld; ++i) a.stats[r * a.stats_ld + i] = i == 1 ? 1.0f : 0.0f;
 }
 
 constexpr long long kWaitCycles = 4000000000ll;  // about 2 s
@@ -454,9 +471,7 @@ __global__ void __launch_bounds__(kRingThreads, KR > 4 ? 1 : 3) distill_kernel(c
         last_w = w;
         ++n;
       } else if (rank == 0 && lane == 0) {
-        a.loss[r] = 0.0f;
-        a.stats[2 * r] = 0.0f;
-        a.stats[2 * r + 1] = 1.0f;
+        write_padding(a, r);
       }
       if (r + stride < rows && next_w != 0.0f) set(RowSlice<T>(a, r + stride, rank, log2c));
       fetch(r + 2 * stride);
@@ -633,11 +648,7 @@ __global__ void __launch_bounds__(NT) distill_wide_kernel(const DistillArgs a) {
   const float w = GRAD ? a.weight[r] : 1.0f;
   if (w == 0.0f) {  // a padding row: not read
     for (int v = sl.v0 + tid; v < sl.v1; v += NT) out_row.store(sl.rv, v, make_uint4(0, 0, 0, 0));
-    if (rank == 0 && tid == 0) {
-      a.loss[r] = 0.0f;
-      a.stats[2 * r] = 0.0f;
-      a.stats[2 * r + 1] = 1.0f;
-    }
+    if (rank == 0 && tid == 0) write_padding(a, r);
     return;
   }
   cl.sync();  // every CTA of the cluster runs: their shared memory is written below
@@ -760,12 +771,14 @@ __global__ void __launch_bounds__(NT) distill_wide_kernel(const DistillArgs a) {
       store_elem<T>(out_row.row, en.id[k], wt * (power2((en.z[k] - sum.ref) * scale) * q_factor - power2(en.p[k])));
 }
 
-// The gradient from a forward pass's stats: one CTA per tile of NT * NV vectors of a row, held in registers.  89 us
+// The gradient from a forward pass's stats: one CTA per tile of NT * NV vectors of a row, held in registers.  90 us
 // for 1024 x 50001 f32 with 100 entries (4.6 TB/s); 239 us with single-number arithmetic and element-wise stores.
-template <typename T, int NT>
+// FULL: six stats a row.
+template <typename T, int NT, bool FULL>
 __global__ void __launch_bounds__(NT, 1024 / NT) distill_grad_kernel(const DistillArgs a, int tiles) {
+  constexpr int NS = FULL ? 6 : 2;
   extern __shared__ uint32_t smem[];
-  __shared__ float p_sum, stat[2];
+  __shared__ float p_sum, stat[NS];
   const long long r = blockIdx.x / tiles;
   const int rank = static_cast<int>(blockIdx.x - r * tiles);
   const int tid = threadIdx.x;
@@ -778,7 +791,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_grad_kernel(const Disti
     for (int v = sl.v0 + tid; v < sl.v1; v += NT) out.store(sl.rv, v, make_uint4(0, 0, 0, 0));
     return;
   }
-  if (tid >= NT - 2) stat[tid - (NT - 2)] = a.stats[2 * r + tid - (NT - 2)];  // (the first threads have entries to fetch)
+  if (tid >= NT - NS) stat[tid - (NT - NS)] = a.stats[NS * r + tid - (NT - NS)];  // (the first threads have entries to fetch)
   sl.load(0);
   Entries en;
   en.id = reinterpret_cast<int*>(smem);
@@ -797,29 +810,40 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_grad_kernel(const Disti
     some |= id >= 0 && !(en.p[k] == neg_inff());
     if (id >= lo && id < hi) en.z[k] = Elem<T>::from_bits(Elem<T>::load_bits(z_row + id));
   }
-  if (a.teacher_lse)
+  if (FULL || a.teacher_lse)
     __syncthreads();
   else
     some = __syncthreads_or(some);
-  const float inv_t = 1.0f / a.temperature, lse = stat[0];
-  float off = stat[1];
-  const bool missing = off == 1.0f;  // the outcome outside S (where it is there, P is 1 but for its rounding)
-  const float P = tid < 32 ? entry_probs<false>(a, en, r, missing) : 0.0f;
-  if (missing) {  // the same for the whole CTA; a closed teacher's P is known without the sum
-    off = some ? 1.0f : 0.0f;
-    if (a.teacher_lse) {
-      if (tid == 0) p_sum = P;
-      __syncthreads();
-      off = p_sum;
+  const float inv_t = 1.0f / a.temperature, wt = w * inv_t;
+  // outside S: f 2^e, e = (z - z_out) log2(e) / T, or (z / T + c) log2(e)
+  float c, f, f_in;  // and f_in, the factor of q_j in S
+  const float scale = kLog2e / a.temperature;
+  if (FULL) {
+    if (tid < 32) entry_probs<false>(a, en, r, false);
+    c = -stat[NS - 2];
+    f = wt * stat[NS - 1];
+    f_in = stat[NS - 3];
+  } else {
+    float off = stat[1];
+    const bool missing = off == 1.0f;  // the outcome outside S (where it is there, P is 1 but for its rounding)
+    const float P = tid < 32 ? entry_probs<false>(a, en, r, missing) : 0.0f;
+    if (missing) {  // the same for the whole CTA; a closed teacher's P is known without the sum
+      off = some ? 1.0f : 0.0f;
+      if (a.teacher_lse) {
+        if (tid == 0) p_sum = P;
+        __syncthreads();
+        off = p_sum;
+      }
     }
+    // where the factor is large, q_j underflows before their product does: it is formed in the exponent
+    const bool fold = !(fabsf(off) < 1024.0f);
+    c = fold ? logf(fabsf(off)) - stat[0] : -stat[0];
+    f = fold ? copysignf(wt, off) : wt * off;
+    f_in = missing ? off : 1.0f;
   }
-  const float wt = w * inv_t;
-  auto q = [&](float z) { return power2((z * inv_t - lse) * kLog2e); };
-  // where the factor is large, q_j underflows before their product does: it is formed in the exponent
-  const bool fold = !(fabsf(off) < 1024.0f);
-  const float c = fold ? logf(fabsf(off)) - lse : -lse, f = fold ? copysignf(wt, off) : wt * off;
-  const float2 inv2 = make_float2(inv_t, inv_t), c2 = make_float2(c, c), log2e2 = make_float2(kLog2e, kLog2e),
-               f2 = make_float2(f, f);
+  const float2 c2 = make_float2(c, c), f2 = make_float2(f, f), inv2 = make_float2(inv_t, inv_t);
+  const float u = FULL ? scale : kLog2e;
+  const float2 u2 = make_float2(u, u);
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int v = sl.vec(0, i);
@@ -827,7 +851,8 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_grad_kernel(const Disti
       uint4 g;
 #pragma unroll
       for (int j = 0; j < Elem<T>::PAIRS; ++j) {
-        const float2 d = mul2(add2(mul2(Elem<T>::pair(sl.r[i], j), inv2), c2), log2e2);
+        const float2 z = Elem<T>::pair(sl.r[i], j);
+        const float2 d = mul2(FULL ? add2(z, c2) : fma2(z, inv2, c2), u2);
         Elem<T>::set_pair(g, j, mul2(make_float2(power2(d.x), power2(d.y)), f2));
       }
       out.store(sl.rv, v, g);
@@ -835,7 +860,10 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_grad_kernel(const Disti
   }
   __syncthreads();
   for (int k = tid; k < a.k; k += NT)
-    if (en.id[k] >= lo && en.id[k] < hi) store_elem<T>(g_row, en.id[k], wt * ((missing ? off : 1.0f) * q(en.z[k]) - en.p[k]));
+    if (en.id[k] >= lo && en.id[k] < hi) {
+      const float e = FULL ? (en.z[k] - stat[NS - 4]) * scale : fmaf(en.z[k], inv_t, -stat[0]) * kLog2e;
+      store_elem<T>(g_row, en.id[k], wt * (f_in * power2(e) - en.p[k]));
+    }
 }
 
 template <typename K>
@@ -881,7 +909,8 @@ cudaError_t launch(const DistillArgs& a, bool with_loss, bool with_grad, int num
   constexpr int NT = 512;
   constexpr long long TILE = NT * NV * 16;
   const int tiles = static_cast<int>((bytes + 32 + TILE - 1) / TILE);
-  distill_grad_kernel<T, NT><<<static_cast<unsigned>(a.x.rows * tiles), NT, static_cast<size_t>(a.k) * 12, s>>>(a, tiles);
+  auto kernel = a.stats_ld == 6 ? distill_grad_kernel<T, NT, true> : distill_grad_kernel<T, NT, false>;
+  kernel<<<static_cast<unsigned>(a.x.rows * tiles), NT, static_cast<size_t>(a.k) * 12, s>>>(a, tiles);
   const cudaError_t e = cudaGetLastError();
   if (e == cudaSuccess) (*launches)++;
   return e;

@@ -45,6 +45,7 @@ struct DistillArgs {
   const float* weight;
   float* loss;
   float* stats;
+  int stats_ld;  // 2 or 6 floats per row
   void* grad;
   long long grad_ld;
   uint32_t* err;

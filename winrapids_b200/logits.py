@@ -68,7 +68,7 @@ def _distill_function():
         @staticmethod
         def forward(logits, values, ids, lse, temperature):
             out = _ctx(logits.device.index).distill_loss(logits, ids, values, teacher_lse=lse, temperature=temperature,
-                                                         sync=False)
+                                                         sync=False, full_stats=True)
             return out["loss"], out["stats"]
 
         @staticmethod
