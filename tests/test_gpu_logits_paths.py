@@ -304,3 +304,43 @@ def test_stats_columns_are_two_or_six(ctx):
     x, teacher = ctx._logits(z), ctx._teacher(ctx._logits(z), ids, t, None, 1.0, 4)
     loss = torch.zeros(2, device="cuda")
     assert ctx._L.tbgb_distill_loss(ctx._h, x, teacher, loss.data_ptr(), loss.data_ptr(), None) == 7
+
+
+# ---- host threads ---------------------------------------------------------------------------------
+
+
+def test_threads_with_tables_of_different_sizes():
+    """Contexts are independent: two host threads launch the same kernels with different amounts of shared memory."""
+    import threading
+
+    import torch
+
+    import winrapids_b200 as wb
+
+    R = 300
+    failed = []
+
+    def work(vocab, k):
+        c = wb.Context(0)
+        try:
+            z = torch.zeros(R, vocab, device="cuda")
+            ids = torch.arange(8, dtype=torch.int32, device="cuda").repeat(R, 1)
+            t, w, u = torch.zeros(R, 8, device="cuda"), torch.ones(R, device="cuda"), torch.zeros(R, device="cuda")
+            out = {"loss": torch.empty(R, device="cuda"), "stats": torch.empty(R, 2, device="cuda")}
+            grad = torch.empty_like(z)
+            for i in range(400):
+                c.distill_step(z, ids, t, w, grad=grad, out=out, sync=i % 100 == 99)
+                c.sample_tokens(z, u, top_k=k, sync=False)
+                c.top_logits(z, k, sync=False)
+            c.sync()
+        except Exception as e:  # noqa: BLE001
+            failed.append(repr(e))
+        finally:
+            c.close()
+
+    threads = [threading.Thread(target=work, args=a) for a in ((7000, 900), (8600, 600), (7800, 1000))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed

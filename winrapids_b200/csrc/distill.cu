@@ -866,13 +866,6 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_grad_kernel(const Disti
     }
 }
 
-template <typename K>
-cudaError_t allow_smem(K kernel, size_t bytes) {
-  return bytes > 48 * 1024
-             ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes))
-             : cudaSuccess;
-}
-
 template <typename T>
 cudaError_t launch(const DistillArgs& a, bool with_loss, bool with_grad, int num_sms, cudaStream_t s,
                    uint64_t* launches) {

@@ -447,6 +447,33 @@ cudaError_t launch_rows(void (*kernel)(P...), int threads, int cluster, size_t s
   return cudaLaunchKernelEx(&l.cfg, kernel, args...);
 }
 
+// Lets `kernel` be launched with `smem` bytes of dynamic shared memory.  The limit belongs to the function, not to a
+// context or a call: it is only ever set to the most that a CTA can have, so no host thread lowers it under another's
+// launch.  (That it is set is kept per thread: setting it costs as long as a launch.)
+template <typename... P>
+cudaError_t allow_smem(void (*kernel)(P...), size_t smem) {
+  if (smem <= 48 * 1024) return cudaSuccess;
+  struct Set {
+    void (*kernel)(P...);
+    int device;
+  };
+  static thread_local Set last[8] = {};
+  static thread_local unsigned next = 0;
+  int device = 0, most = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return e;
+  for (const Set& k : last)
+    if (k.kernel == kernel && k.device == device) return cudaSuccess;
+  cudaFuncAttributes fixed;
+  e = cudaFuncGetAttributes(&fixed, kernel);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&most, cudaDevAttrMaxSharedMemoryPerBlockOptin, device);
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             most - static_cast<int>(fixed.sharedSizeBytes));
+  if (e == cudaSuccess) last[next++ % 8] = Set{kernel, device};
+  return e;
+}
+
 // Clusters of a persistent kernel that the device holds at once.  A cluster lies within one GPC, so
 // this is less than the SMs' room divided by its size (C = 8: 48 instead of 55), and one cluster
 // more than it would run after the others: twice the time.
@@ -469,10 +496,8 @@ cudaError_t resident_clusters(void (*kernel)(P...), int threads, int cluster, si
       *n = k.n;
       return cudaSuccess;
     }
-  if (smem > 48 * 1024) {
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-    if (e != cudaSuccess) return e;
-  }
+  e = allow_smem(kernel, smem);
+  if (e != cudaSuccess) return e;
   ClusterLaunch l(threads, cluster, smem, 1, nullptr);
   e = cudaOccupancyMaxActiveClusters(n, kernel, &l.cfg);
   if (e == cudaSuccess) last[next++ % 8] = Asked{kernel, device, cluster, smem, *n};

@@ -900,10 +900,8 @@ cudaError_t launch(const SampleArgs& a, int num_sms, cudaStream_t s) {
   smem = std::max(smem, sizeof(ExactSmem));
   smem = std::max(smem, static_cast<size_t>(kPartBytes) + (c > 1 ? 2 : 1) * kEdgeMost * 8);
   auto kernel = a.mask ? sample_kernel<T, NT, true> : sample_kernel<T, NT, false>;
-  if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-    if (e != cudaSuccess) return e;
-  }
+  const cudaError_t e = allow_smem(kernel, smem);
+  if (e != cudaSuccess) return e;
   return launch_rows(kernel, NT, c, smem, a.x.rows, s, a, list_k);
 }
 

@@ -291,10 +291,8 @@ cudaError_t launch(const TopArgs& a, int num_sms, cudaStream_t s) {
   const size_t lists = (static_cast<size_t>(top_vec_cap(a.k)) + top_el_cap(a.k)) * 8;
   const size_t smem = lists > sizeof(ExactSmem) ? lists : sizeof(ExactSmem);
   auto kernel = a.mask ? top_logits_kernel<T, NT, true> : top_logits_kernel<T, NT, false>;
-  if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-    if (e != cudaSuccess) return e;
-  }
+  const cudaError_t e = allow_smem(kernel, smem);
+  if (e != cudaSuccess) return e;
   return launch_rows(kernel, NT, c, smem, a.x.rows, s, a);
 }
 
