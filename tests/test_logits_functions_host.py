@@ -1,0 +1,69 @@
+"""The functions of winrapids_b200/logits.py without a device: what they hand to a context, and when."""
+import threading
+import time
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+import winrapids_b200 as wb  # noqa: E402
+from winrapids_b200 import logits as module  # noqa: E402
+
+
+class FakeContext:
+    """Takes calls as a Context does; notes the ones that overlap."""
+
+    made = 0
+
+    def __init__(self, device):
+        type(self).made += 1
+        self.inside, self.overlaps, self.calls = 0, 0, []
+        time.sleep(0.01)
+
+    def _enter(self, name, args, kwargs):
+        self.overlaps += self.inside > 0
+        self.inside += 1
+        time.sleep(0.001)
+        self.inside -= 1
+        self.calls.append((name, args, kwargs))
+
+    def top_logits(self, z, k, **kw):
+        self._enter("top_logits", (z, k), kw)
+        rows = z.shape[0]
+        return {"values": torch.zeros(rows, k), "ids": torch.zeros(rows, k, dtype=torch.int32), "lse": torch.zeros(rows)}
+
+    def sample_tokens(self, z, u, **kw):
+        self._enter("sample_tokens", (z, u), kw)
+        rows = z.shape[0]
+        return {"tokens": torch.zeros(rows, dtype=torch.int32), "logprobs": torch.zeros(rows)}
+
+
+@pytest.fixture
+def fake(monkeypatch):
+    FakeContext.made = 0
+    monkeypatch.setattr(module, "Context", FakeContext)
+    monkeypatch.setattr(module, "_CTX", {})
+    monkeypatch.setattr(module, "_device", lambda z: 0)
+    return module._CTX
+
+
+def test_one_call_at_a_time_on_the_shared_context(fake):
+    def work():
+        for _ in range(10):
+            wb.top_logits(torch.zeros(2, 3, 5), 2)
+            wb.sample_tokens(torch.zeros(2, 5), torch.zeros(2))
+
+    threads = [threading.Thread(target=work) for _ in range(6)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert FakeContext.made == 1
+    assert len(fake[0].calls) == 120 and fake[0].overlaps == 0
+
+
+def test_logits_on_the_host_are_refused():
+    for f in (lambda z: wb.top_logits(z, 2), lambda z: wb.sample_tokens(z, torch.zeros(2)),
+              lambda z: wb.distill_loss(z, wb.TopLogits(z[:, :2], z[:, :2].int(), None, 1.0))):
+        with pytest.raises(wb.InvalidArgument):
+            f(torch.zeros(2, 5))

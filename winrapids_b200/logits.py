@@ -9,23 +9,40 @@ tbgb_sample_tokens) for logits of any leading shape [..., vocab] on the device:
 
 They enqueue on torch's current stream and do not wait; ``synchronize(device)`` waits and raises
 what the device reported (a token id outside the vocabulary, an id named twice in a record).
+
+They may be called from any host thread (a backward pass runs on one of autograd's): the context that they
+share per device takes one call at a time.
 """
 from __future__ import annotations
 
+import threading
 from dataclasses import dataclass
 
-from . import InvalidArgument, _torch
+from . import Context, InvalidArgument, _torch
+
+_LOCK = threading.Lock()
+_CTX: dict[int, Context] = {}
 
 
-def _ctx(device: int):
-    from .frame import _ctx as frame_ctx
+def _call(device: int, method: str, *args, **kwargs):
+    """Context.<method> on the device's context, alone."""
+    with _LOCK:
+        if device not in _CTX:
+            _CTX[device] = Context(device)
+        return getattr(_CTX[device], method)(*args, **kwargs)
 
-    return frame_ctx(device)
+
+def _device(logits) -> int:
+    if not isinstance(logits, _torch().Tensor) or not logits.is_cuda:
+        raise InvalidArgument(7, "logits must be a tensor on a CUDA device")
+    return logits.get_device()
 
 
 def synchronize(device: int = 0):
     """Wait for torch's current stream on `device` and raise what the kernels reported."""
-    _ctx(device).sync(_torch().cuda.current_stream(device))
+    stream = _torch().cuda.current_stream(device)
+    stream.synchronize()  # (not while other threads' calls wait for the context)
+    _call(device, "sync", stream)
 
 
 def _rows(t):
@@ -57,7 +74,7 @@ class TopLogits:
 def top_logits(logits, k: int, temperature: float = 1.0, mask=None) -> TopLogits:
     """The record of a teacher's logits [..., vocab]."""
     lead = logits.shape[:-1]
-    out = _ctx(logits.device.index).top_logits(_rows(logits), k, temperature=temperature, mask=mask, sync=False)
+    out = _call(_device(logits), "top_logits", _rows(logits), k, temperature=temperature, mask=mask, sync=False)
     return TopLogits(out["values"].view(*lead, k), out["ids"].view(*lead, k), out["lse"].view(lead), float(temperature))
 
 
@@ -67,8 +84,8 @@ def _distill_function():
     class DistillLoss(torch.autograd.Function):
         @staticmethod
         def forward(logits, values, ids, lse, temperature):
-            out = _ctx(logits.device.index).distill_loss(logits, ids, values, teacher_lse=lse, temperature=temperature,
-                                                         sync=False, full_stats=True)
+            out = _call(_device(logits), "distill_loss", logits, ids, values, teacher_lse=lse, temperature=temperature,
+                        sync=False, full_stats=True)
             return out["loss"], out["stats"]
 
         @staticmethod
@@ -81,8 +98,8 @@ def _distill_function():
         @torch.autograd.function.once_differentiable
         def backward(ctx, grad_loss, _):
             logits, values, ids, lse, stats = ctx.saved_tensors
-            grad = _ctx(logits.device.index).distill_grad(logits, ids, values, stats, grad_loss.float().contiguous(),
-                                                          teacher_lse=lse, temperature=ctx.temperature, sync=False)
+            grad = _call(_device(logits), "distill_grad", logits, ids, values, stats, grad_loss.float().contiguous(),
+                         teacher_lse=lse, temperature=ctx.temperature, sync=False)
             return grad, None, None, None, None
 
     return DistillLoss
@@ -112,8 +129,8 @@ def sample_tokens(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, mas
     def flat(v, dtype):
         return v.reshape(-1).to(dtype) if isinstance(v, torch.Tensor) else v
 
-    out = _ctx(logits.device.index).sample_tokens(
-        _rows(logits), flat(u, torch.float32), temperature=flat(temperature, torch.float32),
+    out = _call(
+        _device(logits), "sample_tokens", _rows(logits), flat(u, torch.float32), temperature=flat(temperature, torch.float32),
         top_k=flat(top_k, torch.int32), top_p=flat(top_p, torch.float32), min_p=flat(min_p, torch.float32), mask=mask,
         sync=False)
     return out["tokens"].view(lead), out["logprobs"].view(lead)
