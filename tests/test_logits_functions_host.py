@@ -67,3 +67,22 @@ def test_logits_on_the_host_are_refused():
               lambda z: wb.distill_loss(z, wb.TopLogits(z[:, :2], z[:, :2].int(), None, 1.0))):
         with pytest.raises(wb.InvalidArgument):
             f(torch.zeros(2, 5))
+
+
+def test_masks_take_the_leading_shape(fake):
+    z, u = torch.zeros(2, 3, 130), torch.zeros(2, 3)
+    words = torch.arange(18).view(2, 3, 3)
+    wb.top_logits(z, 2, mask=words)
+    wb.sample_tokens(z, u, mask=words)
+    wb.top_logits(z, 2, mask=words[0, 0])
+    wb.sample_tokens(z[0], u[0], mask=words[0])
+    wb.sample_tokens(z[0, 0], u[0, 0], mask=words[0, 0])
+    wb.sample_tokens(z, u, mask=words.view(6, 3))
+    got = [c[2]["mask"] for c in fake[0].calls]
+    assert torch.equal(got[5], words.view(6, 3))
+    assert torch.equal(got[0], words.view(6, 3)) and torch.equal(got[1], words.view(6, 3))
+    assert torch.equal(got[2], words[0, 0]) and torch.equal(got[3], words[0]) and torch.equal(got[4], words[0, 0])
+    with pytest.raises(wb.InvalidArgument):
+        wb.top_logits(z, 2, mask=words[:, :2])
+    with pytest.raises(wb.InvalidArgument):
+        wb.sample_tokens(z, u, mask=words.view(3, 2, 3))

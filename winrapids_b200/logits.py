@@ -55,6 +55,15 @@ def _rows(t):
         raise InvalidArgument(7, "the leading dimensions must be viewable as one (make the tensor contiguous)") from None
 
 
+def _mask(mask, logits):
+    """A token mask as the library takes it: [words] for every position, or [rows, words]."""
+    if mask is None or mask.dim() <= 2:
+        return mask
+    if mask.shape[:-1] != logits.shape[:-1]:
+        raise InvalidArgument(7, f"mask has leading shape {tuple(mask.shape[:-1])}, logits {tuple(logits.shape[:-1])}")
+    return _rows(mask)
+
+
 @dataclass
 class TopLogits:
     """A teacher's record: per position the k largest logits (values) with their token ids, the
@@ -72,9 +81,10 @@ class TopLogits:
 
 
 def top_logits(logits, k: int, temperature: float = 1.0, mask=None) -> TopLogits:
-    """The record of a teacher's logits [..., vocab]."""
+    """The record of a teacher's logits [..., vocab].  mask: words of the vocabulary [words] for every position, or
+    [..., words]."""
     lead = logits.shape[:-1]
-    out = _call(_device(logits), "top_logits", _rows(logits), k, temperature=temperature, mask=mask, sync=False)
+    out = _call(_device(logits), "top_logits", _rows(logits), k, temperature=temperature, mask=_mask(mask, logits), sync=False)
     return TopLogits(out["values"].view(*lead, k), out["ids"].view(*lead, k), out["lse"].view(lead), float(temperature))
 
 
@@ -122,7 +132,7 @@ def distill_loss(logits, record: TopLogits):
 
 def sample_tokens(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, mask=None):
     """(tokens int32, log-probabilities f32) of the leading shape, from uniform numbers u of that shape.
-    The settings are numbers or tensors of that shape; see Context.sample_tokens."""
+    The settings are numbers or tensors of that shape, mask is [words] or [..., words]; see Context.sample_tokens."""
     torch = _torch()
     lead = logits.shape[:-1]
 
@@ -131,6 +141,6 @@ def sample_tokens(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, mas
 
     out = _call(
         _device(logits), "sample_tokens", _rows(logits), flat(u, torch.float32), temperature=flat(temperature, torch.float32),
-        top_k=flat(top_k, torch.int32), top_p=flat(top_p, torch.float32), min_p=flat(min_p, torch.float32), mask=mask,
-        sync=False)
+        top_k=flat(top_k, torch.int32), top_p=flat(top_p, torch.float32), min_p=flat(min_p, torch.float32),
+        mask=_mask(mask, logits), sync=False)
     return out["tokens"].view(lead), out["logprobs"].view(lead)
