@@ -86,3 +86,26 @@ def test_masks_take_the_leading_shape(fake):
         wb.top_logits(z, 2, mask=words[:, :2])
     with pytest.raises(wb.InvalidArgument):
         wb.sample_tokens(z, u, mask=words.view(3, 2, 3))
+
+
+def test_k_past_32_bits_is_no_other_k(fake):
+    z, u = torch.zeros(3, 130), torch.zeros(3)
+    wb.sample_tokens(z, u, top_k=torch.tensor([7, 2 ** 32 + 5, -2 ** 32 + 3]))
+    assert fake[0].calls[0][2]["top_k"].tolist() == [7, 2 ** 31 - 1, 0]
+
+
+@pytest.mark.parametrize("k,want", [(5, 5), (2 ** 32 + 5, 2 ** 31 - 1), (-2 ** 32 + 3, 0), (2 ** 31, 2 ** 31 - 1)])
+def test_a_number_k_past_32_bits_is_no_other_k(monkeypatch, k, want):
+    seen = []
+
+    class Library:
+        def tbgb_sample_tokens(self, h, x, u, p, *rest):
+            seen.append(p.top_k_all)
+            return 0
+
+    c = wb.Context.__new__(wb.Context)
+    c._L, c._h, c.device, c._dev = Library(), None, 0, torch.device("cpu")
+    monkeypatch.setattr(wb.Context, "_check_tensor", lambda self, t, what, dtypes: None)
+    monkeypatch.setattr(wb, "_current_stream", lambda device: 0)
+    c.sample_tokens(torch.zeros(2, 9), torch.zeros(2), top_k=k, sync=False)
+    assert seen == [want]

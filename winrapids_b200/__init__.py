@@ -547,7 +547,7 @@ class Context:
         if isinstance(top_k, torch.Tensor):
             p.top_k = self._row_vector(top_k, "top_k", torch.int32, rows)
         else:
-            p.top_k_all = int(top_k)
+            p.top_k_all = min(max(int(top_k), 0), 0x7FFFFFFF)  # (a wider number would be cut to its low bits)
         if isinstance(top_p, torch.Tensor):
             p.top_p = self._row_vector(top_p, "top_p", torch.float32, rows)
         else:

@@ -137,7 +137,11 @@ def sample_tokens(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, mas
     lead = logits.shape[:-1]
 
     def flat(v, dtype):
-        return v.reshape(-1).to(dtype) if isinstance(v, torch.Tensor) else v
+        if not isinstance(v, torch.Tensor):
+            return v
+        if dtype == torch.int32 and v.dtype == torch.int64:  # (a wider number would be cut to its low bits)
+            v = v.clamp(0, 0x7FFFFFFF)
+        return v.reshape(-1).to(dtype)
 
     out = _call(
         _device(logits), "sample_tokens", _rows(logits), flat(u, torch.float32), temperature=flat(temperature, torch.float32),
