@@ -104,8 +104,31 @@ def test_a_number_k_past_32_bits_is_no_other_k(monkeypatch, k, want):
             return 0
 
     c = wb.Context.__new__(wb.Context)
-    c._L, c._h, c.device, c._dev = Library(), None, 0, torch.device("cpu")
+    c._L, c._h, c.device, c._torch_dev = Library(), None, 0, torch.device("cpu")
     monkeypatch.setattr(wb.Context, "_check_tensor", lambda self, t, what, dtypes: None)
     monkeypatch.setattr(wb, "_current_stream", lambda device: 0)
     c.sample_tokens(torch.zeros(2, 9), torch.zeros(2), top_k=k, sync=False)
     assert seen == [want]
+
+
+def test_a_context_does_not_need_torch():
+    """Only the calls that make tensors do."""
+    import subprocess
+    import sys
+
+    program = """
+import sys
+sys.modules["torch"] = None  # an import of it fails
+import winrapids_b200 as wb
+
+class Library:
+    def tbgb_create(self, device, handle): return 0
+    def tbgb_destroy(self, handle): return 0
+
+wb.lib = Library
+c = wb.Context(0)
+c.close()
+print("made")
+"""
+    got = subprocess.run([sys.executable, "-c", program], capture_output=True, text=True, timeout=120)
+    assert got.stdout.strip() == "made", got.stderr

@@ -85,7 +85,7 @@ class Context:
             raise error_for(st, f"tbgb_create(device={device}) failed (an sm_100 device is required)")
         self._h = h
         self.device = int(device)
-        self._dev = _torch().device("cuda", self.device)
+        self._torch_dev = None
 
     def close(self):
         if getattr(self, "_h", None):
@@ -381,6 +381,13 @@ class Context:
         if not t.is_contiguous():
             raise InvalidArgument(7, f"{what} must be contiguous")
         return t.data_ptr()
+
+    @property
+    def _dev(self):
+        """torch's name of the device (a context alone does not need torch)."""
+        if self._torch_dev is None:
+            self._torch_dev = _torch().device("cuda", self.device)
+        return self._torch_dev
 
     def _out(self, out, name: str, dtype, shape):
         t = out.get(name) if out else None
