@@ -344,3 +344,77 @@ def test_threads_with_tables_of_different_sizes():
     for t in threads:
         t.join()
     assert not failed
+
+
+# ---- many rows, long rows --------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("rows,vocab,dtype,k", [(2000, 4099, "f32", 20), (2000, 4099, "bf16", 20), (600, 50001, "f16", 64),
+                                                (600, 50001, "f32", 100), (700, 4099, "bf16", 200)])
+def test_distill_more_rows_than_clusters(ctx, rows, vocab, dtype, k, tail):
+    """Each cluster takes several rows: every stage, barrier phase and part is used again, padding rows (which are
+    not counted there) lie between others."""
+    import torch
+
+    z = table(rows, vocab, dtype, rows, spread=1.5)
+    ids, t, lse = record(z, k, 1.0, 3, dtype, tail)
+    weight = torch.rand(rows, generator=torch.Generator().manual_seed(5)) + 0.5
+    weight[torch.rand(rows, generator=torch.Generator().manual_seed(6)) < 0.2] = 0.0
+    weight[-1] = 0.0
+    weight = weight.cuda()
+    a, g, b = check_rows(ctx, z, ids, t, lse, 1.0, dtype, weight=weight)
+    in_place = z.clone()
+    c = ctx.distill_step(in_place, ids, t, weight, teacher_lse=lse, grad=in_place)
+    assert torch.equal(in_place, b["grad"]) and torch.equal(c["loss"], b["loss"])
+
+
+@pytest.mark.parametrize("dtype", DT)
+def test_top_logits_of_long_rows_on_one_cta(ctx, dtype):
+    from test_gpu_logits import check_top
+
+    import torch
+
+    z = table(80, 50001, dtype, 71)
+    for k in (1, 64, 1000):
+        check_top(ctx, z, k)
+    bits = np.random.default_rng(0).random((80, 50001)) < 0.3
+    words = torch.from_numpy(np.stack([ref.pack_mask(b) for b in bits])).cuda()
+    check_top(ctx, z, 20, T=0.7, mask=words, bits=bits)
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("setting", [dict(), dict(mp=0.05), dict(p=0.9), dict(k=40), dict(k=1000, p=0.95), dict(T=0.0)],
+                         ids=str)
+def test_sampling_of_long_rows_on_one_cta(ctx, dtype, setting):
+    z = table(150, 50001, dtype, 81, spread=2.0)
+    check_sample(ctx, z, uniform(150, 4), **setting)
+
+
+@pytest.mark.parametrize("dtype", DT)
+def test_sampling_of_long_masked_rows_on_one_cta(ctx, dtype):
+    import torch
+
+    z = table(150, 20001, dtype, 82, spread=2.0)
+    bits = np.random.default_rng(1).random((150, 20001)) < 0.1
+    words = torch.from_numpy(np.stack([ref.pack_mask(b) for b in bits])).cuda()
+    for s in (dict(), dict(p=0.9), dict(k=50)):
+        check_sample(ctx, z, uniform(150, 5), mask=words, bits=bits, **s)
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("rows,vocab", [(4, 70001), (150, 9001)])
+def test_k_past_the_lists_with_top_p(ctx, rows, vocab, dtype):
+    z = table(rows, vocab, dtype, 83)
+    for s in (dict(k=3000, p=0.8), dict(k=1025, p=0.3), dict(k=vocab, p=0.7), dict(k=vocab - 1, mp=0.01)):
+        check_sample(ctx, z, uniform(rows, 6), **s)
+
+
+@pytest.mark.parametrize("rows", [2, 150])
+def test_top_p_whose_end_lies_among_thousands_of_equal_logits(ctx, rows):
+    """More equal logits at the end of the prefix than the quick way lists."""
+    import torch
+
+    z = (table(1, 60000, "f32", 84, spread=2.0) * 2).round().div(2).bfloat16()
+    for p in (0.5, 0.9, 0.99):
+        check_sample(ctx, z.expand(rows, 60000), uniform(rows, 7), p=p)
