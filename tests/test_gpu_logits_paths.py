@@ -418,3 +418,14 @@ def test_top_p_whose_end_lies_among_thousands_of_equal_logits(ctx, rows):
     z = (table(1, 60000, "f32", 84, spread=2.0) * 2).round().div(2).bfloat16()
     for p in (0.5, 0.9, 0.99):
         check_sample(ctx, z.expand(rows, 60000), uniform(rows, 7), p=p)
+
+
+@pytest.mark.parametrize("dtype", DT)
+def test_few_rows_with_a_k_of_their_own(ctx, dtype):
+    """Lists of up to 1024 on several CTAs a row, as many as the lists hold."""
+    import torch
+
+    z = table(6, 70001, dtype, 85)
+    k = torch.tensor([1024, 1000, 700, 300, 1, 0], dtype=torch.int32, device="cuda")
+    p = torch.tensor([1.0, 0.5, 0.9, 1.0, 0.3, 0.9], device="cuda")
+    check_sample(ctx, z, uniform(6, 8), k=k, p=p)

@@ -891,10 +891,12 @@ cudaError_t launch(const SampleArgs& a, int num_sms, cudaStream_t s) {
   const long long nvec = static_cast<long long>(a.x.vocab) * sizeof(T) / 16 + 2;
   // the lists of the k largest: for the k of all rows where it is one, for every k they can hold where rows have their own
   const int list_k = a.p.top_k ? kTopMax : std::min(std::max(a.p.top_k_all, 1), kTopMax);
-  const int often_k = a.p.top_k ? 256 : list_k;  // (a larger k on several CTAs may spill: the exact row)
-  // more CTAs for a row while rows leave SMs without work, a lane keeps a step and the lists hold them all
+  // More CTAs for a row while rows leave SMs without work, a lane keeps a step and the lists hold what all the CTAs may
+  // collect (a row that spills takes the exact way: 32 x 131072 with rows' own k up to 1024 500 us with four CTAs, 91 with
+  // two).  Two CTAs an SM in all: 64 x 150001 f32 top-p 68 us (one: 80, four: 103, always one a row: 125), 100 x 131072
+  // uncut 27 (30, 32, 30); top-k alone would do with fewer (64 rows: 24, 19, 46, 18).
   int c = 1;
-  auto more = [&] { return c < 8 && nvec / (c * 2) >= NT && c * 2 * often_k * 5 / 4 + 64 < top_el_cap(list_k); };
+  auto more = [&] { return c < 8 && nvec / (c * 2) >= NT && c * 2 * list_k * 5 / 4 + 64 < top_el_cap(list_k); };
   while (more() && a.x.rows * c * 2 <= 2 * num_sms) c *= 2;
   size_t smem = (static_cast<size_t>(top_vec_cap(list_k)) + top_el_cap(list_k)) * 8;
   smem = std::max(smem, sizeof(ExactSmem));
