@@ -871,7 +871,9 @@ cudaError_t launch(const DistillArgs& a, bool with_loss, bool with_grad, int num
                    uint64_t* launches) {
   const long long bytes = static_cast<long long>(a.x.vocab) * sizeof(T);
   if (with_loss) {
-    // the fewest CTAs whose two stages leave room for three CTAs on an SM, more while rows are few
+    // The fewest CTAs whose two stages leave room for three CTAs on an SM: 4096 x 131072 bf16 step 484 us (as many as fit one
+    // CTA: 746), 2048 x 100003 f16 loss 129 (room for two: 150, for one: 170); 600 x 50001 f32 would do with two (54, not 61).
+    // More while rows are few, up to two CTAs an SM in all: 64 x 32000 bf16 step 7.7 us (never: 7.9, up to four: 10.4).
     const bool aligned = reinterpret_cast<uintptr_t>(a.x.logits) % 16 == 0 && a.x.ld * sizeof(T) % 16 == 0;
     const long long nvec = aligned ? (bytes + 15) / 16 : bytes / 16 + 2;
     int c = 1;
@@ -880,6 +882,8 @@ cudaError_t launch(const DistillArgs& a, bool with_loss, bool with_grad, int num
     const long long cap = (nvec + c - 1) / c * 16;
     if (2 * cap <= 222 * 1024) {
       const size_t smem = static_cast<size_t>(2 * cap);
+      // Entries stay in the registers of their warp, 4 a lane, or 32 for long records, which leaves room for one CTA an SM:
+      // 512 x 131072 bf16 step with K 64 69 us (in the kernel for 32: 429), K 128 73 (485), K 129 483, K 1024 978.
       auto kernel = a.k <= 128 ? (with_grad ? distill_kernel<T, 4, true> : distill_kernel<T, 4, false>)
                                : (with_grad ? distill_kernel<T, 32, true> : distill_kernel<T, 32, false>);
       int held = 0;

@@ -4,8 +4,8 @@
 // With zmax the row's largest allowed logit, a token's weight is
 //   w = 2^((z - zmax) * (log2(e) / T)),   rounded to a multiple of 2^-30,
 // so weights are whole numbers (in units of 2^-30, at most 2^30 each) and every sum of them is
-// exact: the token does not depend on the order of summation, on the split over CTAs or on the
-// hardware.  The grid is finer than the numbers that pick (a 32-bit uniform number has steps of
+// exact: the token does not depend on the order of summation or on the split over CTAs.  (The power itself is the
+// device's ex2.approx, right to about 2 units in the last place of 24 bits.)  The grid is finer than the numbers that pick (a 32-bit uniform number has steps of
 // 2^-24) and than the rounding of a 32-bit running sum would be.
 //   top-k   the first k by (logit descending, id ascending)
 //   top-p   of those, with sum W, the shortest prefix whose sum reaches ceil(p W)

@@ -20,7 +20,7 @@ using namespace row;
 
 struct ExactSmem {
   SelectSmem sel;
-  unsigned long long list[kTopMax];
+  alignas(16) unsigned long long list[kTopMax];
   float wm[32], ws[32];
   float2 cta_ms;
   int warp_ties[32], cta_ties, n_list;
@@ -151,25 +151,8 @@ __device__ __noinline__ void exact_row(const TopArgs& a, long long r, ExactSmem&
   cl.sync();
   if (rank != 0) return;
 
-  // sort the list (at most K entries), largest first
   const int n = min(n_list, a.k);
-  int n2 = 1;
-  while (n2 < n) n2 <<= 1;
-  for (int j = n + tid; j < n2; j += NT) list[j] = 0;
-  __syncthreads();
-  for (int size = 2; size <= n2; size <<= 1)
-    for (int step = size >> 1; step > 0; step >>= 1) {
-      for (int p = tid; p < n2 / 2; p += NT) {
-        const int i = (p / step) * step * 2 + p % step, j = i + step;
-        const bool down = (i & size) == 0;
-        const unsigned long long x = list[i], y = list[j];
-        if ((x < y) == down) {
-          list[i] = y;
-          list[j] = x;
-        }
-      }
-      __syncthreads();
-    }
+  sort_list<NT>(list, n);
   for (int j = tid; j < a.k; j += NT) {
     const bool have = j < n;
     const long long o = r * a.k + j;
@@ -285,7 +268,9 @@ template <typename T>
 cudaError_t launch(const TopArgs& a, int num_sms, cudaStream_t s) {
   constexpr int NT = 256;
   const long long nvec = static_cast<long long>(a.x.vocab) * sizeof(T) / 16 + 2;
-  // more CTAs for a row while rows leave SMs without work, a lane keeps a step and the lists hold them all
+  // More CTAs for a row while rows leave SMs without work, a lane keeps a step and the lists hold them all: 60 x 50001 f32
+  // 16 us (always one: 18, up to two or four an SM: 17, 24), 30 x 131072 bf16 with K 200 25 (31, 25, 25); 8 x 32000 bf16,
+  // where the clusters' barriers cost as much as the rows, 14 (13).
   int c = 1;
   while (c < 8 && a.x.rows * c * 2 <= num_sms && nvec / (c * 2) >= NT && c * 2 * a.k * 5 / 4 + 64 < top_el_cap(a.k)) c *= 2;
   const size_t lists = (static_cast<size_t>(top_vec_cap(a.k)) + top_el_cap(a.k)) * 8;
