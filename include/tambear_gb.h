@@ -405,8 +405,9 @@ tbgb_status tbgb_distill_loss(tbgb_ctx* ctx, const tbgb_logits* x, const tbgb_te
 tbgb_status tbgb_distill_grad(tbgb_ctx* ctx, const tbgb_logits* x, const tbgb_teacher* teacher,
                               const float* d_stats, const float* d_weight, void* d_grad, int64_t grad_stride,
                               void* stream);
-/* Both in one pass over the logits, for weights known beforehand.  A row with weight 0 is padding: it
- * is not read, its loss and gradient are 0 and its stats (0, 1). */
+/* Both, for weights known beforehand, in one pass over the logits (rows past about 227,000 F32 or 454,000 16-bit
+ * logits: two).  A row with weight 0 is padding: it is not read, its loss and gradient are 0 and its
+ * stats (0, 1) (and zeros). */
 tbgb_status tbgb_distill_step(tbgb_ctx* ctx, const tbgb_logits* x, const tbgb_teacher* teacher,
                               const float* d_weight, float* d_loss, float* d_stats, void* d_grad,
                               int64_t grad_stride, void* stream);

@@ -79,6 +79,8 @@ struct GradRow {
 
 // ---- loss and stats, and the gradient, in one pass over the logits -----------------------------------
 //
+// For rows that the stages of a cluster of eight hold (222 KB a CTA for two of them: 227,000 32-bit or 454,000 16-bit
+// logits); longer ones below take two passes.
 // One cluster per row at a time, persistent over rows; CTA c holds its slice of a row in one of two
 // stages of shared memory.  Warp roles:
 //   producer   bulk-copies the slice of the next row as soon as its stage is free
@@ -95,6 +97,8 @@ __device__ __forceinline__ float scaled(float m, float s, float top, float scale
   return m == neg_inff() || m == top ? s : s * power2((m - top) * scale);
 }
 
+// 1 / total and the factors are quotients right to 2 units of the last place: 1.2e-7 of a gradient that the powers of two
+// leave with 2.4e-7 and more.
 struct RowPart {  // a CTA's part of a row
   float m, s;     // largest logit outside S, sum of 2^((z - m) * scale)
   float ms, ss;   // the same over S
@@ -631,7 +635,8 @@ __device__ __forceinline__ float entry_probs(const DistillArgs& a, const Entries
 }
 
 // Rows too long for the stages above: a cluster per row, the slices read in tiles, a bit per element of the
-// slice for the entries; the gradient in a second pass over the slice.
+// slice for the entries; the gradient in a second pass over the slice.  512 x 524288 bf16: loss 356 us (1.5 TB/s), step
+// 561 us (1.9 TB/s of what it reads and writes once): one CTA an SM, bound by its latencies.
 template <typename T, int NT, bool GRAD>
 __global__ void __launch_bounds__(NT) distill_wide_kernel(const DistillArgs a) {
   constexpr int NW = NT / 32, EPV = Elem<T>::EPV;
@@ -772,8 +777,8 @@ __global__ void __launch_bounds__(NT) distill_wide_kernel(const DistillArgs a) {
 }
 
 // The gradient from a forward pass's stats: one CTA per tile of NT * NV vectors of a row, held in registers.  90 us
-// for 1024 x 50001 f32 with 100 entries (4.6 TB/s); 239 us with single-number arithmetic and element-wise stores.
-// FULL: six stats a row.
+// for 1024 x 50001 f32 with 100 entries (4.6 TB/s), 75 with 8: the stores wait behind a barrier for the entries (the barrier is
+// the largest stall); 239 us with single-number arithmetic and element-wise stores.  FULL: six stats a row, 85 us.
 template <typename T, int NT, bool FULL>
 __global__ void __launch_bounds__(NT, 1024 / NT) distill_grad_kernel(const DistillArgs a, int tiles) {
   constexpr int NS = FULL ? 6 : 2;

@@ -291,13 +291,15 @@ __device__ __noinline__ void exact_row(const SampleArgs& a, long long r, ExactSm
 // 2^-7 + e has steps of 2^-30, so its bits less those of 2^-7 are e in those units (rounded to nearest,
 // ties to even, as the conversion does), and bits are summed.  A conversion would cost a second
 // instruction on the special function units, which are busy for most of the pass with the power itself.
-// 96 us for 1024 x 100000 bf16 uncut (2.1 TB/s of its first pass's bytes), 115 for top-p alone and 31 for top-k with top-p
-// over 256 x 131072 bf16; 512 threads a row (256: 197 and 34 us, 1024: 130 and 47).
+// 96 us for 1024 x 100000 bf16 uncut (2.1 TB/s of its first pass's bytes); 149 for top-p 0.95 alone, 29 for top-k with top-p
+// and 24 greedy over 256 x 131072 bf16.  512 threads a row: 256 took 1.7 times as long for top-p, 1024 1.1 and 1.5 times for
+// top-p and top-k.
 
 constexpr int kParts = 1024;       // of the exponent's range
 constexpr int kPartBytes = 9 * 1024;  // two words for each, later the search's arrays
-// Tokens of the part that holds the end of the prefix: equal 16-bit logits between 16 and 32 are up to one in 30 of a
-// vocabulary with a spread of 2.
+// Tokens of the part that holds the end of the prefix; with more the row takes the exact way.  Equal 16-bit logits between
+// 16 and 32 are up to one in 40 of a vocabulary with a spread of 2: 256 rows of 151936 bf16 logits around 20, top-p 0.95,
+// 229 us (around 0: 189), of 201088 9.4 ms (246).  A longer list costs the CTAs that an SM holds.
 constexpr int kEdgeMost = 4096;
 constexpr float kSmall = 0.0078125f;  // 2^-7
 

@@ -4,9 +4,10 @@
 //                 is clear are never taken, and a row with fewer ends in (-inf, -1)
 //   lse           log sum exp(z / T) over the logits that are neither NaN nor masked
 //
-// 166 us for the 64 largest of 2048 x 131072 bf16 (3.2 TB/s), 41 us for 20 of 509 x 50001 f32 (2.5 TB/s): bound by
-// instructions (11.7 an element, 5 of them the softmax) and the fixed work per row, which four CTAs of 256
-// threads an SM hide better than two of 512 (210 us).
+// 165 us for the 64 largest of 2048 x 131072 bf16 (3.3 TB/s), 39 us for 20 of 509 x 50001 f32 (2.6 TB/s): bound by
+// instructions (11.3 an element, 5 of them the softmax) and the fixed work per row, which four CTAs of 256
+// threads an SM hide better than two of 512 (210 us).  A mask of its own per row takes the element-wise loads:
+// 512 x 131072 bf16 52 us, masked 103.
 #include <climits>
 
 #include "logits_select.cuh"
