@@ -259,9 +259,6 @@ struct RowSlice {
     w1 = nv > 0 && (rv.off + rv.vocab) % Elem<T>::EPV && v0 + nv == rv.nvec ? nv - 1 : nv;
   }
   __device__ __forceinline__ const char* at(int j) const { return rv.base + static_cast<long long>(v0 + j) * 16; }
-  __device__ __forceinline__ uint4 load(int j) const {
-    return j >= w0 && j < w1 ? __ldcs(reinterpret_cast<const uint4*>(at(j))) : rv.load_part(v0 + j);
-  }
 };
 
 // Warps of the third role: what a warp does once a row (waits, reductions, the cluster's sums) is about 500 instructions,
@@ -590,8 +587,8 @@ __global__ void __launch_bounds__(kRingThreads, KR > 4 ? 1 : 3) distill_kernel(c
   cl.sync();
 }
 
-// The row's entries in shared memory: id (-1: none, also an id outside the vocabulary, which is
-// reported), student logit (only of ids in [lo, hi), or of all when `all`), teacher probability.
+// The row's entries in shared memory: id (-1: none, also an id outside the vocabulary, which is reported), student
+// logit (of ids in this CTA's part [lo, hi)), the teacher's logit, then p or log2 p.
 struct Entries {
   int* id;
   float* z;
